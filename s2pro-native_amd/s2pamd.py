@@ -120,6 +120,25 @@ class SpecBuffers(ctypes.Structure):
                 ("replans", I)]
 
 
+class PagePool(ctypes.Structure):
+    """s2p_page_pool (include/s2pro/paged.h)"""
+    _fields_ = [("kv", P), ("scales", P), ("layers", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page", ctypes.c_int32), ("bits", ctypes.c_int32)]
+
+
+class PageBatch(ctypes.Structure):
+    """s2p_page_batch (include/s2pro/paged.h)"""
+    _fields_ = [("table", P), ("len", P), ("row0", P), ("sessions", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("max_rows", ctypes.c_int32), ("max_len", ctypes.c_int32)]
+
+
+class PageTables(ctypes.Structure):
+    """s2p_page_tables (include/s2pro/paged.h)"""
+    _fields_ = [("ref", P), ("table", P), ("held", P), ("len", P), ("sessions", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/s2pro/*.h
 SIGS = {
     # status.h / tensor.h
@@ -187,6 +206,19 @@ SIGS = {
     "s2pk_sample": (I, [P, I64, P, P, I, P, P, P, P, P]),
     "s2pk_embed": (I, [P, P, P, I, I, P]),
     "s2pk_argmax": (I, [P, P, I, I, P]),
+    # paged.h
+    "s2p_page_pool_bytes": (SZ, [P]),
+    "s2p_page_pool_scale_bytes": (SZ, [P]),
+    "s2pk_rope_table": (I, [P, I, I, F, P]),
+    "s2pk_paged_append": (I, [P, P, I, P, I, P, P, F, P, I, P, P, P]),
+    "s2pk_paged_attention": (I, [P, P, I, P, I, P, P, P, P]),
+    "s2pk_paged_attention_work_floats": (I64, [P, I, I]),
+    "s2pk_paged_commit": (I, [P, P, P, P, P, P]),
+    "s2pk_pages_work_ints": (I64, [P, P]),
+    "s2pk_pages_reserve": (I, [P, P, P, P, P, P]),
+    "s2pk_pages_fork": (I, [P, P, P, P, I, P, P]),
+    "s2pk_pages_free": (I, [P, P, P, P]),
+    "s2pk_pages_compact": (I, [P, P, P, P, P]),
     # fastar.h
     "s2pfa_create": (I, [P, P, I, P]),
     "s2pfa_create_random": (I, [P, I, I, U64, P]),
