@@ -552,6 +552,7 @@ def _bind(st):
                                 max_pages=st["width"])
         n = lib.s2pk_pages_work_ints(ctypes.byref(b["pool"]), ctypes.byref(b["tab"]))
         b["work"] = torch.empty(n, dtype=torch.int32, device=DEV)
+        b["live"] = torch.zeros((), dtype=torch.int64, device=DEV)  # the call writes its low word
     b["pool_p"] = ctypes.byref(b["pool"])
     b["batch_p"] = ctypes.byref(b["batch"]) if "batch" in b else None
     b["tab_p"] = ctypes.byref(b["tab"]) if "tab" in b else None
@@ -586,7 +587,7 @@ def _own_run(st):
         m.hip_check(lib.s2pk_pages_reserve(b["pool_p"], b["tab_p"], st["want"].data_ptr(),
                                            granted.data_ptr(), b["work"].data_ptr(), s), "reserve")
         return {"state": st["state"], "granted": granted, "kv": st["kv"]}
-    live = torch.empty((), dtype=torch.int32, device=DEV)
+    live = b["live"]
     m.hip_check(lib.s2pk_pages_free(b["pool_p"], b["tab_p"], st["keep"].data_ptr(), s), "free")
     m.hip_check(lib.s2pk_pages_compact(b["pool_p"], b["tab_p"], live.data_ptr(),
                                        b["work"].data_ptr(), s), "compact")
