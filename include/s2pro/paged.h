@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define S2P_PAGE_MAX_SESSIONS 1024 /* of s2p_page_tables */
+#define S2P_PAGE_MAX_SESSIONS 1024 /* of a batch, of the tables */
 #define S2P_PAGED_MAX_GROUP 16     /* query heads a kv head */
 
 typedef struct {
@@ -54,7 +54,8 @@ typedef struct {
     const int32_t* table;  /* [sessions][max_pages] */
     const int32_t* len;    /* [sessions] tokens before this call's rows */
     const int32_t* row0;   /* [sessions + 1] */
-    int32_t sessions, max_pages;
+    int32_t sessions;      /* <= S2P_PAGE_MAX_SESSIONS */
+    int32_t max_pages;
     int32_t rows;          /* of the row arrays */
     int32_t max_rows;      /* host bound of a session's rows */
     int32_t max_len;       /* host bound of len + rows, <= max_pages * page */

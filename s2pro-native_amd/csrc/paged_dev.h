@@ -22,7 +22,7 @@ static inline bool pg_pool_ok(const s2p_page_pool* p) {
 }
 static inline bool pg_batch_ok(const s2p_page_pool* p, const s2p_page_batch* b) {
     if (!b || !b->table || !b->len || !b->row0) return false;
-    if (b->sessions <= 0 || b->sessions > 65535 || b->max_pages <= 0) return false;
+    if (b->sessions <= 0 || b->sessions > S2P_PAGE_MAX_SESSIONS || b->max_pages <= 0) return false;
     if (b->max_rows <= 0 || b->max_rows > b->max_len) return false;
     return (int64_t)b->max_len <= (int64_t)b->max_pages * p->page;
 }

@@ -35,7 +35,7 @@ BAD_POOL = [dict(kv=None), dict(kv=A + 8), dict(bits=5), dict(bits=8), dict(bits
             dict(pages=0), dict(pages=-1), dict(pages=(1 << 28) + 1), dict(kv_heads=0),
             dict(kv_heads=2000)]
 BAD_BATCH = [dict(table=None), dict(len=None), dict(row0=None), dict(sessions=0),
-             dict(sessions=70000), dict(max_pages=0), dict(max_rows=0), dict(max_len=0),
+             dict(sessions=1025), dict(max_pages=0), dict(max_rows=0), dict(max_len=0),
              dict(max_len=65), dict(max_rows=65, max_len=64)]
 BAD_TABLES = [dict(ref=None), dict(table=None), dict(held=None), dict(len=None), dict(sessions=0),
               dict(sessions=1025), dict(max_pages=0)]
