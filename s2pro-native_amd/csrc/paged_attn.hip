@@ -32,8 +32,9 @@ struct PgAttn {
     const uint64_t* vis;
     uint16_t* out;
     float* work;
+    int* sums; /* [sessions] rounds up to each (the merge's view of the schedule) */
     int qh, kvh, g;
-    int nb; /* blocks a kv head that share the rounds */
+    int nb, nvt; /* blocks a kv head that share the rounds, for each tile of query vectors */
 };
 
 template <int BW>
@@ -122,16 +123,64 @@ S2P_DEV void pd_swap32(uint32_t& a, uint32_t& b) { /* a's upper half wave <-> b'
 S2P_DEV float pd_half(uint32_t w, int hi) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(hi ? w >> 16 : w & 0xFFFFu));
 }
-/* transposing reads: in a 16-lane group lane 2 r + h gives the address of 8 bytes, row r,
- * columns 8 h .. + 7, and lane i gets column i of rows 0 .. 7 (4 bits: lane r gives row r's 16
- * columns, lane i gets column i of rows 0 .. 15, row 0 in the lowest nibble) */
-S2P_DEV s2p_u32x2 pd_tr8(const LDS(unsigned char)* p) {
-    typedef __attribute__((__vector_size__(2 * sizeof(int)))) int i2;
-    return __builtin_bit_cast(s2p_u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS(i2)*)p));
+/* two floats as a bf16 pair, one conversion for both */
+S2P_DEV uint32_t pd_pk(float a, float b) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f2;
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 b2;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
 }
-S2P_DEV s2p_u32x2 pd_tr4(const LDS(unsigned char)* p) {
-    typedef __attribute__((__vector_size__(2 * sizeof(int)))) int i2;
-    return __builtin_bit_cast(s2p_u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((LDS(i2)*)p));
+/* LDS reads of what global_load_lds wrote.  In C++ each would wait for every load in flight, the
+ * next tile's too (the compiler does not tell the buffers apart), so they are written out, each
+ * block with its own wait; what they read has arrived by pd_wait. */
+S2P_DEV uint32_t pd_lds(const LDS(unsigned char)* p) { return (uint32_t)(uintptr_t)p; }
+/* the transposing ones: in a 16-lane group lane 4 r + h gives the address of 8 bytes, row r,
+ * columns 4 h .. + 3, and lane i gets column i of rows 0 .. 3 (16 bits); 8 bits: lane 2 r + h,
+ * columns 8 h .. + 7, rows 0 .. 7; 4 bits: lane r, 16 columns, rows 0 .. 15, row 0 lowest */
+template <int O>
+S2P_DEV void pd_tr16(uint32_t a, uint32_t b, s2p_u32x2& x0, s2p_u32x2& x1, s2p_u32x2& y0,
+                     s2p_u32x2& y1) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4\n"
+        "ds_read_b64_tr_b16 %1, %4 offset:%6\n"
+        "ds_read_b64_tr_b16 %2, %5\n"
+        "ds_read_b64_tr_b16 %3, %5 offset:%6\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x0), "=&v"(x1), "=&v"(y0), "=&v"(y1) : "v"(a), "v"(b), "n"(O) : "memory");
+}
+S2P_DEV void pd_tr4(uint32_t a, s2p_u32x2& x, s2p_u32x2& y) {
+    asm volatile(
+        "ds_read_b64_tr_b4 %0, %2\n"
+        "ds_read_b64_tr_b4 %1, %2 offset:8\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x), "=&v"(y) : "v"(a) : "memory");
+}
+/* 32 bytes: four slots' scales */
+template <int O>
+S2P_DEV void pd_scales4(uint32_t a, s2p_u32x4& x, s2p_u32x4& y) {
+    asm volatile(
+        "ds_read_b128 %0, %2 offset:%3\n"
+        "ds_read_b128 %1, %2 offset:%4\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x), "=&v"(y) : "v"(a), "n"(O), "n"(O + 16) : "memory");
+}
+/* of slots 0 .. 3 and 16 .. 19 the scales of two groups (a dword): x[p][0, 1], x[p][2, 3] */
+template <int G>
+S2P_DEV void pd_scales8(uint32_t a, s2p_u32x2 (&x)[2][2]) {
+    asm volatile(
+        "ds_read2_b32 %0, %4 offset0:%5 offset1:%5+2\n"
+        "ds_read2_b32 %1, %4 offset0:%5+4 offset1:%5+6\n"
+        "ds_read2_b32 %2, %4 offset0:%5+32 offset1:%5+34\n"
+        "ds_read2_b32 %3, %4 offset0:%5+36 offset1:%5+38\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1])
+        : "v"(a), "n"(G) : "memory");
+}
+S2P_DEV void pd_tr8(uint32_t a, uint32_t b, s2p_u32x2& x, s2p_u32x2& y) {
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %2\n"
+        "ds_read_b64_tr_b8 %1, %3\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x), "=&v"(y) : "v"(a), "v"(b) : "memory");
 }
 /* the loads of the tile before the last N have arrived */
 template <int N>
@@ -158,36 +207,46 @@ S2P_DEV uint64_t pd_groups(int bad) {
 /* the waves' O in LDS: 16-byte pieces of a vector's row permuted (rows lie a bank apart) */
 S2P_DEV int pd_oidx(int vec, int d) { return vec * PG_HD + ((((d >> 2) ^ vec) & 15) << 2) + (d & 64) + (d & 3); }
 
-/* rounds of `rnd` slots of the sessions, summed up to each in s_pre; returns all.  Every thread
- * of the block (of 256 or more) calls it. */
-S2P_DEV int pd_rounds(const PgAttn& a, int rnd, int* s_pre, int* s_w) {
+/* The batch as a block keeps it in LDS: a session's rounds summed up with those before it, its
+ * first row, length and rows. */
+struct PdBatch {
+    int pre[S2P_PAGE_MAX_SESSIONS], r0[S2P_PAGE_MAX_SESSIONS], len[S2P_PAGE_MAX_SESSIONS];
+    uint8_t n[S2P_PAGE_MAX_SESSIONS]; /* max_rows is at most 32 here */
+    int w[PD_WAVES];
+};
+/* Fills it (256 threads); returns all rounds of `rnd` slots. */
+S2P_DEV int pd_batch(const PgAttn& a, int rnd, PdBatch& b) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    constexpr int E = S2P_PAGE_MAX_SESSIONS / 256; /* neighbouring sessions a thread */
-    int v[E], sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int s = tid * E + e;
+    int before = 0;
+    for (int base = 0; base < a.b.sessions; base += 64 * PD_WAVES) {
+        const int s = base + tid;
+        int v = 0;
         if (s < a.b.sessions) {
             const PgSess ss = pg_session(a.b, s);
-            if (ss.n > 0) sum += (ss.L + ss.n + rnd - 1) / rnd;
+            if (ss.n > 0) v = (ss.L + ss.n + rnd - 1) / rnd;
+            b.r0[s] = ss.r0;
+            b.len[s] = ss.L;
+            b.n[s] = (uint8_t)ss.n;
         }
-        v[e] = sum;
-    }
-    int up = sum;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(up, o, 64);
-        if (lane >= o) up += t;
-    }
-    if (lane == 63) s_w[wave] = up;
-    __syncthreads();
-    up -= sum;
-    for (int w = 0; w < wave; w++) up += s_w[w];
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(v, o, 64);
+            if (lane >= o) v += t;
+        }
+        if (base) __syncthreads(); /* w is read no more */
+        if (lane == 63) b.w[wave] = v;
+        __syncthreads();
+        int all = before;
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        if (tid < 256) s_pre[tid * E + e] = up + v[e];
+        for (int w = 0; w < PD_WAVES; w++) {
+            if (w < wave) v += b.w[w];
+            all += b.w[w];
+        }
+        if (s < a.b.sessions) b.pre[s] = before + v;
+        before = all;
+    }
     __syncthreads();
-    return s_pre[a.b.sessions - 1];
+    return before;
 }
 
 /* A bf16 tile that not every row sees whole: V rows that are not there become zeros (what lies
@@ -258,41 +317,44 @@ S2P_DEV void pd_tail(const PgSess& ss, LDS(unsigned char)* vb, int tb, int bad,
  * 16-byte chunks are permuted so that the transposing reads spread over the banks */
 template <int BW>
 struct PdTile {
-    static constexpr int TS = BW == 16 ? 32 : 64, NG = TS / 16;
+    static constexpr int TS = BW == 4 ? 64 : 32, NG = TS / 16;
     static constexpr int EL = BW == 16 ? 256 : BW == 8 ? 128 : 64;
     static constexpr int NP = TS / 16;                          /* MFMAs of 16 slots */
     static constexpr int NK = BW == 16 ? 4 : BW == 8 ? 2 : 1;   /* 16-byte K loads a 16 slots */
     static constexpr int NV = TS * EL / 1024;                   /* 1 KB V loads */
-    static constexpr int VB = TS * EL + (BW == 16 ? 0 : 1024);  /* a buffer: V, then K and V scales */
+    static constexpr int VB = TS * EL + (BW == 16 ? 0 : 16 * TS);  /* a buffer: V, then K and V scales */
     s2p_u32x4 k[NP][NK];
 };
 
 template <int BW>
-S2P_DEV int pd_swz(int t) {
+S2P_DEV unsigned pd_swz(unsigned t) {
     if constexpr (BW == 16) return (t & 7) << 1;
     else if constexpr (BW == 8) return ((t >> 1) & 3) | (((t >> 4) & 1) << 2);
     else return (t >> 4) & 3;
 }
 
 template <int BW, int MQT>
-__global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
+__global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(PgAttn a) {
 #pragma clang fp contract(off)
     typedef PdTile<BW> Tile;
     constexpr int TS = Tile::TS, NG = Tile::NG, NP = Tile::NP, EL = Tile::EL, VB = Tile::VB;
     constexpr int RND = TS * PD_WAVES;
     constexpr int OB = PD_WAVES * 16 * MQT * PG_HD * 4;
     constexpr int VBUF = PD_WAVES * 2 * VB;
-    __shared__ __align__(16) unsigned char s_buf[VBUF > OB ? VBUF : OB];
+    __shared__ __align__(256) unsigned char s_buf[VBUF > OB ? VBUF : OB];
     __shared__ float s_ml[PD_WAVES][16 * MQT][2];
-    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[PD_WAVES];
+    __shared__ PdBatch s_b;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qq = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x % a.kvh, blk = blockIdx.x / a.kvh;
+    const int kvh = blockIdx.x % a.kvh, vt = blockIdx.x / a.kvh % a.nvt;
+    const int blk = blockIdx.x / a.kvh / a.nvt, v0 = 16 * MQT * vt; /* vectors from v0 on */
     LDS(unsigned char)* const vbuf = (LDS(unsigned char)*)s_buf + wave * 2 * VB;
 
     /* the block's share of the rounds of all sessions */
-    const int total = pd_rounds(a, RND, s_pre, s_w);
+    const int total = pd_batch(a, RND, s_b);
+    if (blockIdx.x == 0) /* for the merge */
+        for (int i = tid; i < a.b.sessions; i += 64 * PD_WAVES) a.sums[i] = s_b.pre[i];
     const int nb = min(a.nb, total); /* every one of them has a round */
     if (blk >= nb) return;
     const int begin = (int)((int64_t)blk * total / nb);
@@ -300,8 +362,8 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
     int vrow[MQT], vhead[MQT];
 #pragma unroll
     for (int qt = 0; qt < MQT; qt++) {
-        vrow[qt] = (16 * qt + c) / a.g;
-        vhead[qt] = kvh * a.g + (16 * qt + c) % a.g;
+        vrow[qt] = (v0 + 16 * qt + c) / a.g;
+        vhead[qt] = kvh * a.g + (v0 + 16 * qt + c) % a.g;
     }
 
     for (int cur = begin; cur < end;) {
@@ -309,13 +371,16 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
         int s = 0, hi = a.b.sessions - 1;
         while (s < hi) {
             const int mid = (s + hi) >> 1;
-            if (s_pre[mid] > cur) hi = mid;
+            if (s_b.pre[mid] > cur) hi = mid;
             else s = mid + 1;
         }
         s = __builtin_amdgcn_readfirstlane(s);
-        const int first = __builtin_amdgcn_readfirstlane(s ? s_pre[s - 1] : 0);
-        const int last = __builtin_amdgcn_readfirstlane(s_pre[s]);
-        const PgSess ss = pg_session(a.b, s);
+        const int first = __builtin_amdgcn_readfirstlane(s ? s_b.pre[s - 1] : 0);
+        const int last = __builtin_amdgcn_readfirstlane(s_b.pre[s]);
+        PgSess ss;
+        ss.r0 = __builtin_amdgcn_readfirstlane(s_b.r0[s]);
+        ss.n = __builtin_amdgcn_readfirstlane((int)s_b.n[s]);
+        ss.L = __builtin_amdgcn_readfirstlane(s_b.len[s]);
         const int span = ss.L + ss.n;
         const int stop = min(end, last);
         const int p0 = (cur - first) * RND, p1 = min((stop - first) * RND, span);
@@ -342,8 +407,8 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
         }
         /* deq_int4 gives 1.5 + code / 16: a second product takes the 1.5 off (in registers of
          * their own its sums would cost 16 a vector tile) */
-        const s2p_u32x4 k15 = {0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};
-        (void)k15;
+        s2p_u32x4 k15 = {0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};
+        if (BW == 4) asm volatile("" : "+v"(k15)); /* kept, not made again for every product */
         /* m (in units of log2), l (this lane's slots), o: O^T, dims 16 dt + 4 qq + v of
          * vector 16 qt + c */
         float m[MQT], l[MQT];
@@ -358,8 +423,9 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
             for (int dt = 0; dt < 8; dt++) o[qt][dt] = (s2p_f32x4){0.f, 0.f, 0.f, 0.f};
         }
 
+        const int nvec = min(16 * MQT, ss.n * a.g - v0); /* of this tile; may be none */
         const int tb0 = p0 + wave * TS;
-        const int n = tb0 < p1 ? (p1 - tb0 + RND - 1) / RND : 0;
+        const int n = nvec > 0 && tb0 < p1 ? (p1 - tb0 + RND - 1) / RND : 0;
         int ids = 0; /* lane x: the page of the wave's 16-slot group x (of 64 / NG tiles), or -1 */
         auto page_ids = [&](int k) __attribute__((always_inline)) {
             const int slot = tb0 + (k + lane / NG) * RND + 16 * (lane % NG);
@@ -374,9 +440,9 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
          * reads page 0 and is masked. */
         auto issue = [&](Tile& t, int k) __attribute__((always_inline)) {
             if ((k & (64 / NG - 1)) == 0) page_ids(k);
-            int lane = threadIdx.x & 63; /* offsets made here, not kept through the loop */
+            unsigned lane = threadIdx.x & 63; /* offsets made here, not kept through the loop */
             asm volatile("" : "+v"(lane));
-            const int c = lane & 15, qq = lane >> 4;
+            const unsigned c = lane & 15, qq = lane >> 4;
             const int tb = tb0 + k * RND, x0 = (k & (64 / NG - 1)) * NG;
             LDS(unsigned char)* const vb = vbuf + (k & 1) * VB;
             uint64_t at[NG];
@@ -388,13 +454,15 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
             }
             const uint64_t vplane = (uint64_t)(uint32_t)a.kvh << a.l.shift;
             if constexpr (BW != 16) {
-                /* lanes 0..31: two slots' K scales each, 32..63: their V scales */
-                const int g = (lane >> 3) & 3;
-                const uint64_t sa = (g & 2 ? (g & 1 ? at[3] : at[2]) : (g & 1 ? at[1] : at[0])) +
-                                    (lane & 32 ? vplane : 0);
-                __builtin_amdgcn_global_load_lds(
-                    (PgGlb*)((GblPtr)(uint64_t)a.l.sc + sa * 8 + 16 * (lane & 7)),
-                    (PgLds*)(vb + TS * EL), 16, 0, 0);
+                /* two slots' scales a lane: K's in the first TS / 2 lanes, then V's */
+                const int g = (lane >> 3) & (NG - 1);
+                uint64_t sa = g & 1 ? at[1] : at[0];
+                if (NG == 4) sa = g & 2 ? (g & 1 ? at[NG - 1] : at[NG - 2]) : sa;
+                if (lane & (TS / 2)) sa += vplane;
+                if (TS == 64 || lane < TS)
+                    __builtin_amdgcn_global_load_lds(
+                        (PgGlb*)((GblPtr)(uint64_t)a.l.sc + sa * 8 + 16 * (lane & 7)),
+                        (PgLds*)(vb + TS * EL), 16, 0, 0);
             }
 #pragma unroll
             for (int p = 0; p < NP; p++) {
@@ -406,9 +474,9 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
 #pragma unroll
             for (int i = 0; i < Tile::NV; i++) {
                 const int g = i * (1024 / EL) / 16; /* the load's rows lie in one group */
-                const int t0 = i * (1024 / EL) % 16, tl = lane / (EL / 16);
+                const unsigned t0 = i * (1024 / EL) % 16, tl = lane / (EL / 16);
                 const GblPtr vp = gbl_base(a.l.kv, (at[g] + vplane) * EL);
-                const int ch = (lane % (EL / 16)) ^ pd_swz<BW>(i * (1024 / EL) + tl);
+                const unsigned ch = (lane % (EL / 16)) ^ pd_swz<BW>(i * (1024 / EL) + tl);
                 __builtin_amdgcn_global_load_lds(
                     (PgGlb*)(vp + (uint32_t)((t0 + tl) * EL + 16 * ch)),
                     (PgLds*)(vb + i * 1024), 16, 0, 2 /* nontemporal */);
@@ -421,13 +489,90 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
             const uint64_t b = __ballot(ids < 0);
             return (int)((b >> ((k & (64 / NG - 1)) * NG)) & ((1u << NG) - 1));
         };
+        /* O^T += V^T P^T over codes: p times a group's V scale is the weight of its 32 dims */
+        [[maybe_unused]] auto codes_pv = [&](const LDS(unsigned char)* vb, float (&x)[MQT][NP][4],
+                                             const uint64_t (&seen)[MQT], auto open)
+                                             __attribute__((always_inline)) {
+            constexpr int NH = NP / 2; /* products of 32 slots */
+            int lane = threadIdx.x & 63;
+            asm volatile("" : "+v"(lane));
+            const int c = lane & 15, qq = lane >> 4;
+            uint32_t mask = 0x00780078u, one = 0x3F803F80u;
+            asm volatile("" : "+v"(mask), "+v"(one));
+            const uint32_t v0 = pd_lds(vb), s0 = v0 + TS * EL + 8 * TS + 32 * qq;
+            /* the row that the lane's address of a transposing read stands for */
+            const int r = BW == 8 ? 16 * (c >> 3) + 4 * qq + ((c >> 1) & 3)
+                                  : 16 * (c >> 2) + 4 * qq + (c & 3);
+            const uint32_t va0 = v0 + r * EL + (pd_swz<BW>(r) << 4) + (BW == 8 ? 8 * (c & 1) : 0);
+            s2p_u32x2 vs[NH][2][2];
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                /* V scales of the lane's slots, groups g and g ^ 1 */
+                if (g == 0) {
+                    pd_scales8<0>(s0, vs[0]);
+                    if constexpr (NH > 1) pd_scales8<64>(s0, vs[NH - 1]);
+                } else if (g == 2) {
+                    pd_scales8<1>(s0, vs[0]);
+                    if constexpr (NH > 1) pd_scales8<65>(s0, vs[NH - 1]);
+                }
+                s2p_u32x2 b[2]; /* V codes: dims 32 g + c, 32 g + 16 + c */
+                if constexpr (BW == 8) pd_tr8(va0 ^ (g << 5), va0 ^ (g << 5) ^ 16, b[0], b[1]);
+                else pd_tr4(va0 ^ (g << 4), b[0], b[1]);
+                s2p_u32x4 w[MQT][NH]; /* the group's weights p vs in bf16 */
+#pragma unroll
+                for (int qt = 0; qt < MQT; qt++)
+#pragma unroll
+                    for (int h = 0; h < NH; h++) {
+                        float y[2][4];
+#pragma unroll
+                        for (int p = 0; p < 2; p++)
+#pragma unroll
+                            for (int v = 0; v < 4; v++)
+                                y[p][v] = fmaf(pd_half(vs[h][p][v >> 1][v & 1], g & 1),
+                                               x[qt][2 * h + p][v], 0.f);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            /* word k: INT8 slots in order, INT4 the order of deq_int4 */
+                            const int p0 = BW == 8 ? k >> 1 : 0, e0 = BW == 8 ? 2 * (k & 1) : k;
+                            const int p1 = BW == 8 ? p0 : 1, e1 = BW == 8 ? e0 + 1 : k;
+                            w[qt][h][k] = pd_pk(y[p0][e0], y[p1][e1]);
+                            if constexpr (!decltype(open)::value) {
+                                /* a scale may be NaN where the slot is not seen */
+                                const uint64_t z = seen[qt] >> (4 * qq + 32 * h);
+                                w[qt][h][k] &= ((z >> (16 * p0 + e0)) & 1 ? 0xFFFFu : 0u) |
+                                               ((z >> (16 * p1 + e1)) & 1 ? 0xFFFF0000u : 0u);
+                            }
+                        }
+                    }
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    s2p_u32x4 va[NH];
+                    if constexpr (BW == 8) {
+                        const s2p_u32x2 u = deq_s8(b[d].x), z = deq_s8(b[d].y);
+                        va[0] = (s2p_u32x4){u.x, u.y, z.x, z.y};
+                    } else {
+                        va[0] = deq_int4(b[d].x, mask, one);
+                        va[NH - 1] = deq_int4(b[d].y, mask, one);
+                    }
+#pragma unroll
+                    for (int qt = 0; qt < MQT; qt++)
+#pragma unroll
+                        for (int h = 0; h < NH; h++) {
+                            if constexpr (BW == 4)
+                                o[qt][2 * g + d] = mfma16x16x32(k15, w[qt][h], o[qt][2 * g + d]);
+                            o[qt][2 * g + d] = mfma16x16x32(va[h], w[qt][h], o[qt][2 * g + d]);
+                        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         auto step = [&](Tile& t, int k, int bad) __attribute__((always_inline)) {
             int lane = threadIdx.x & 63;
             asm volatile("" : "+v"(lane));
             const int c = lane & 15, qq = lane >> 4;
             const int tb = tb0 + k * RND;
             const LDS(unsigned char)* vb = vbuf + (k & 1) * VB;
-            if constexpr (BW != 16) pd_wait<Tile::NV>(); /* the scales, issued before K and V */
+            if constexpr (BW != 16) pd_wait<Tile::NV>(); /* K and the scales, issued before V */
             /* scores of slots tb + 16 p + 4 qq + v, vector 16 qt + c */
             float x[MQT][NP][4];
 #pragma unroll
@@ -467,9 +612,12 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
                     uint32_t mask = 0x00780078u, one = 0x3F803F80u;
                     asm volatile("" : "+v"(mask), "+v"(one));
                     /* K scales of slots 16 p + 4 qq + 0 .. 3, four groups each */
-                    const LDS(s2p_u32x4)* kp =
-                        (const LDS(s2p_u32x4)*)(vb + TS * EL + 8 * (16 * p + 4 * qq));
-                    const s2p_u32x4 ks[2] = {kp[0], kp[1]};
+                    s2p_u32x4 ks[2];
+                    const uint32_t sa = pd_lds(vb) + TS * EL + 32 * qq;
+                    if (p == 0) pd_scales4<0>(sa, ks[0], ks[1]);
+                    else if (p == 1) pd_scales4<128>(sa, ks[0], ks[1]);
+                    else if (p == 2) pd_scales4<256>(sa, ks[0], ks[1]);
+                    else pd_scales4<384>(sa, ks[0], ks[1]);
 #pragma unroll
                     for (int qt = 0; qt < MQT; qt++)
 #pragma unroll
@@ -521,7 +669,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
                 uint64_t see = ~0ull;
                 if (!open) {
                     see = pd_mask(word[qt], ss.L - tb) & pd_groups(bad);
-                    if (TS == 32) see &= 0xFFFFFFFFull;
+                    if (TS == 32) see &= 0xFFFFFFFFull; /* what lies behind the tile */
                     seen[qt] = see;
                     const uint32_t w[2] = {(uint32_t)see >> (4 * qq), (uint32_t)(see >> 32) >> (4 * qq)};
 #pragma unroll
@@ -562,107 +710,28 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
                 for (int qt = 0; qt < MQT; qt++)
 #pragma unroll
                     for (int p = 0; p < 2; p++) {
-                        pw[qt][2 * p] = pk_bf(x[qt][p][0], x[qt][p][1]);
-                        pw[qt][2 * p + 1] = pk_bf(x[qt][p][2], x[qt][p][3]);
+                        pw[qt][2 * p] = pd_pk(x[qt][p][0], x[qt][p][1]);
+                        pw[qt][2 * p + 1] = pd_pk(x[qt][p][2], x[qt][p][3]);
                     }
+                /* rows 4 qq + c / 4 (and + 16), dims 16 dt + 4 (c % 4) */
+                const int r = 4 * qq + (c >> 2);
+                const uint32_t va0 = pd_lds(vb) + r * 256 + ((((c >> 1) & 1) ^ pd_swz<16>(r)) << 4) +
+                                     8 * (c & 1);
 #pragma unroll
-                for (int dt = 0; dt < 8; dt++) {
-                    const int k4 = c >> 2, m4 = c & 3;
-                    s2p_u32x2 b[2];
+                for (int d2 = 0; d2 < 4; d2++) {
+                    s2p_u32x2 b[4];
+                    pd_tr16<4096>(va0 ^ (d2 << 6), va0 ^ (d2 << 6) ^ 32, b[0], b[1], b[2], b[3]);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int r = 16 * h + 4 * qq + k4, d = 16 * dt + 4 * m4;
-                        b[h] = ds_read_tr16((const LDS(uint16_t)*)(vb + r * 256 +
-                                                                   (((d >> 3) ^ pd_swz<16>(r)) << 4) +
-                                                                   2 * (d & 7)));
-                    }
-                    const s2p_u32x4 va = {b[0].x, b[0].y, b[1].x, b[1].y};
-#pragma unroll
-                    for (int qt = 0; qt < MQT; qt++)
-                        o[qt][dt] = mfma16x16x32(va, pw[qt], o[qt][dt]);
-                    if (dt & 1) __builtin_amdgcn_sched_barrier(0);
-                }
-            } else {
-                uint32_t mask = 0x00780078u, one = 0x3F803F80u;
-                asm volatile("" : "+v"(mask), "+v"(one));
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    /* V scales of the lane's slots, groups g and g ^ 1 */
-                    uint32_t vs[NP][4];
-#pragma unroll
-                    for (int p = 0; p < NP; p++)
-#pragma unroll
-                        for (int v = 0; v < 4; v++)
-                            vs[p][v] = *(const LDS(uint32_t)*)(vb + TS * EL + 512 +
-                                                               8 * (16 * p + 4 * qq + v) + 4 * (g >> 1));
-                    /* the group's weights p vs, in bf16, halves h of 32 slots */
-                    s2p_u32x4 w[MQT][2];
-#pragma unroll
-                    for (int qt = 0; qt < MQT; qt++) {
-                        float y[NP][4];
-#pragma unroll
-                        for (int p = 0; p < NP; p++)
-#pragma unroll
-                            for (int v = 0; v < 4; v++)
-                                y[p][v] = x[qt][p][v] * pd_half(vs[p][v], g & 1);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            __builtin_amdgcn_sched_barrier(0);
-                            if constexpr (BW == 8)
-                                w[qt][h] = (s2p_u32x4){pk_bf(y[2 * h][0], y[2 * h][1]),
-                                                       pk_bf(y[2 * h][2], y[2 * h][3]),
-                                                       pk_bf(y[2 * h + 1][0], y[2 * h + 1][1]),
-                                                       pk_bf(y[2 * h + 1][2], y[2 * h + 1][3])};
-                            else
-                                w[qt][h] = (s2p_u32x4){pk_bf(y[2 * h][0], y[2 * h + 1][0]),
-                                                       pk_bf(y[2 * h][1], y[2 * h + 1][1]),
-                                                       pk_bf(y[2 * h][2], y[2 * h + 1][2]),
-                                                       pk_bf(y[2 * h][3], y[2 * h + 1][3])};
-                            if (!open) { /* a scale may be NaN where the slot is not seen */
-#pragma unroll
-                            for (int h = 0; h < 2; h++)
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    /* the word's two slots of the lane */
-                                    const int s0 = BW == 8 ? 32 * h + 16 * (k >> 1) + 2 * (k & 1) : 32 * h + k;
-                                    const int s1 = BW == 8 ? s0 + 1 : s0 + 16;
-                                    const uint64_t z = seen[qt] >> (4 * qq);
-                                    w[qt][h][k] &= ((z >> s0) & 1 ? 0xFFFFu : 0u) |
-                                                   ((z >> s1) & 1 ? 0xFFFF0000u : 0u);
-                                }
-                        }
-                    }
-                    }
-#pragma unroll
-                    for (int d2 = 0; d2 < 2; d2++) {
-                        const int dt = 2 * g + d2;
-                        s2p_u32x4 va[2];
-                        if constexpr (BW == 8) {
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                const int r = c >> 1, t8 = 32 * h + 16 * (r >> 2) + 4 * qq + (r & 3);
-                                const s2p_u32x2 d = pd_tr8(vb + t8 * 128 +
-                                                           ((dt ^ pd_swz<8>(t8)) << 4) + 8 * (c & 1));
-                                const s2p_u32x2 u = deq_s8(d.x), z = deq_s8(d.y);
-                                va[h] = (s2p_u32x4){u.x, u.y, z.x, z.y};
-                            }
-                        } else {
-                            const int t4 = 16 * (c >> 2) + 4 * qq + (c & 3);
-                            const s2p_u32x2 d = pd_tr4(vb + t4 * 64 +
-                                                       (((dt >> 1) ^ pd_swz<4>(t4)) << 4) + 8 * (dt & 1));
-                            va[0] = deq_int4(d.x, mask, one);
-                            va[1] = deq_int4(d.y, mask, one);
-                        }
+                    for (int e = 0; e < 2; e++) {
+                        const s2p_u32x4 va = {b[2 * e].x, b[2 * e].y, b[2 * e + 1].x, b[2 * e + 1].y};
 #pragma unroll
                         for (int qt = 0; qt < MQT; qt++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                if constexpr (BW == 4) o[qt][dt] = mfma16x16x32(k15, w[qt][h], o[qt][dt]);
-                                o[qt][dt] = mfma16x16x32(va[h], w[qt][h], o[qt][dt]);
-                            }
+                            o[qt][2 * d2 + e] = mfma16x16x32(va, pw[qt], o[qt][2 * d2 + e]);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
+            } else {
+                if (open) codes_pv(vb, x, seen, std::true_type());
+                else codes_pv(vb, x, seen, std::false_type());
             }
             return next;
         };
@@ -695,8 +764,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
         __syncthreads();
         /* merge the waves: vector by vector, a dim a thread */
         const bool whole = cur == first && stop == last;
-        const int nvec = min(16 * MQT, ss.n * a.g);
-        float* const po = a.work + ((size_t)(kvh * a.nb + blk) * 2 + (cur == first ? 1 : 0)) *
+        float* const po = a.work + (((size_t)(kvh * a.nb + blk) * 2 + (cur == first ? 1 : 0)) * a.nvt + vt) *
                                        (16 * MQT * (PG_HD + 2));
         for (int i = tid; i < nvec * PG_HD; i += 64 * PD_WAVES) {
             const int vec = i >> 7, d = i & 127;
@@ -713,7 +781,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
                 z = fmaf(so[pd_oidx(w * 16 * MQT + vec, d)], e, z);
             }
             if (whole) {
-                a.out[((size_t)(ss.r0 + vec / a.g) * a.qh + kvh * a.g + vec % a.g) * PG_HD + d] =
+                a.out[((size_t)(ss.r0 + (v0 + vec) / a.g) * a.qh + kvh * a.g + (v0 + vec) % a.g) * PG_HD + d] =
                     f2bf(M == -INFINITY && mark == 0.f ? 0.f : z / lt);
             } else {
                 po[16 * MQT * 2 + i] = z;
@@ -730,35 +798,44 @@ __global__ __launch_bounds__(64 * PD_WAVES, 2) void k_paged_dec(PgAttn a) {
 
 /* Sessions that several blocks worked on: their partials, in the order of the blocks.
  * A block a (vector, kv head, session): four quarters of the blocks, a dim a thread. */
-__global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int rnd, int nvec_max) {
-    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[8];
+__global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int tile) {
     __shared__ float s_m[4], s_l[4], s_k[4], s_z[4][PG_HD];
     const int vec = blockIdx.x, kvh = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, d = tid & 127, part = tid >> 7;
+    const int total = a.sums[a.b.sessions - 1], last = a.sums[s], first = s ? a.sums[s - 1] : 0;
     const PgSess ss = pg_session(a.b, s);
     if (vec >= ss.n * a.g) return;
-    const int total = pd_rounds(a, rnd, s_pre, s_w);
-    const int first = s ? s_pre[s - 1] : 0, last = s_pre[s];
     /* block of a round: the last j whose first round, j total / nb, is not behind it */
     const int nb = min(a.nb, total);
     const int j0 = (int)((((int64_t)first + 1) * nb - 1) / total);
     const int j1 = (int)(((int64_t)last * nb - 1) / total);
     if (j0 == j1) return; /* one block had all of it */
-    const size_t stride = (size_t)nvec_max * (PG_HD + 2);
-    const float* const base = a.work + (size_t)kvh * a.nb * 2 * stride;
+    const size_t stride = (size_t)tile * (PG_HD + 2); /* of a tile's partial */
+    const float* const base = a.work + ((size_t)kvh * a.nb * 2 * a.nvt + vec / tile) * stride;
+    const int tv = vec % tile;
     const int each = (j1 - j0 + 4) >> 2;
     const int from = j0 + part * each, to = min(from + each, j1 + 1);
     float M = -INFINITY, lt = 0.f, z = 0.f, mark = 0.f;
-    for (int j = from; j < to; j++) {
-        const float* p = base + ((size_t)j * 2 + (j == j0 ? 1 : 0)) * stride;
-        const float pm = p[2 * vec], pl = p[2 * vec + 1];
-        const float pz = p[2 * nvec_max + vec * PG_HD + d];
-        const float mn = fmaxf(M, pm), ms = mn == -INFINITY ? 0.f : mn;
-        const float e0 = __builtin_amdgcn_exp2f(M - ms), e1 = __builtin_amdgcn_exp2f(pm - ms);
-        mark = fmaxf(mark, pl);
-        lt = fmaf(lt, e0, pl * e1);
-        z = fmaf(z, e0, pz * e1);
-        M = mn;
+    for (int jj = from; jj < to; jj += 4) { /* four partials' loads at a time */
+        float pm[4], pl[4], pz[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int j = min(jj + u, to - 1);
+            const float* p = base + ((size_t)j * 2 + (j == j0 ? 1 : 0)) * a.nvt * stride;
+            pm[u] = p[2 * tv];
+            pl[u] = p[2 * tv + 1];
+            pz[u] = p[2 * tile + tv * PG_HD + d];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (jj + u >= to) break;
+            const float mn = fmaxf(M, pm[u]), ms = mn == -INFINITY ? 0.f : mn;
+            const float e0 = __builtin_amdgcn_exp2f(M - ms), e1 = __builtin_amdgcn_exp2f(pm[u] - ms);
+            mark = fmaxf(mark, pl[u]);
+            lt = fmaf(lt, e0, pl[u] * e1);
+            z = fmaf(z, e0, pz[u] * e1);
+            M = mn;
+        }
     }
     if (d == 0) {
         s_m[part] = M;
@@ -782,10 +859,11 @@ __global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int rnd, int nvec
         f2bf(M == -INFINITY && mark == 0.f ? 0.f : z / lt);
 }
 
-/* blocks a kv head: two a CU fit, and no more than there are rounds of `rnd` slots */
-static int64_t pd_blocks(const s2p_page_batch* b, int kv_heads, int rnd) {
+/* blocks a kv head and tile of query vectors: as many as fit at once, `each` a CU, and no more
+ * than there are rounds of `rnd` slots */
+static int64_t pd_blocks(const s2p_page_batch* b, int tiles, int rnd, int each) {
     const int64_t most = (int64_t)b->sessions * ((b->max_len + rnd - 1) / rnd);
-    int64_t nb = 2 * s2p_cu_count() / kv_heads;
+    int64_t nb = each * s2p_cu_count() / tiles;
     if (nb < 1) nb = 1;
     return nb < most ? nb : most;
 }
@@ -793,14 +871,15 @@ static int64_t pd_blocks(const s2p_page_batch* b, int kv_heads, int rnd) {
 template <int BW, int MQT>
 static hipError_t pd_launch(PgAttn a, hipStream_t st) {
     const int rnd = PdTile<BW>::TS * PD_WAVES;
-    a.nb = (int)pd_blocks(&a.b, a.kvh, rnd);
-    hipLaunchKernelGGL((k_paged_dec<BW, MQT>), dim3((unsigned)(a.nb * a.kvh)), dim3(64 * PD_WAVES),
-                       0, st, a);
+    a.nvt = (a.b.max_rows * a.g + 16 * MQT - 1) / (16 * MQT);
+    a.nb = (int)pd_blocks(&a.b, a.kvh * a.nvt, rnd, BW == 8 ? 3 : 2);
+    hipLaunchKernelGGL((k_paged_dec<BW, MQT>), dim3((unsigned)(a.nb * a.nvt * a.kvh)),
+                       dim3(64 * PD_WAVES), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nb == 1 || a.b.max_len <= rnd) return e; /* no session is shared */
     hipLaunchKernelGGL(k_paged_merge, dim3((unsigned)(a.b.max_rows * a.g), (unsigned)a.kvh,
                                            (unsigned)a.b.sessions),
-                       dim3(512), 0, st, a, rnd, 16 * MQT);
+                       dim3(512), 0, st, a, 16 * MQT);
     return hipGetLastError();
 }
 
@@ -810,8 +889,9 @@ extern "C" int64_t s2pk_paged_attention_work_floats(const s2p_page_batch* batch,
         !pg_group(q_heads, kv_heads))
         return 0;
     const int vecs = batch->max_rows * pg_group(q_heads, kv_heads);
-    if (vecs > 32) return 4;
-    return kv_heads * pd_blocks(batch, kv_heads, 128) * 2 * (vecs > 16 ? 32 : 16) * (PG_HD + 2) + 4;
+    const int64_t sums = (batch->sessions + 3) & ~3;
+    if (vecs > 32) return sums;
+    return sums + kv_heads * pd_blocks(batch, kv_heads, 128, 3) * 2 * (vecs > 16 ? 32 : 16) * (PG_HD + 2);
 }
 
 extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_page_batch* batch,
@@ -830,7 +910,8 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
     a.q = (const uint16_t*)q;
     a.vis = vis;
     a.out = (uint16_t*)out;
-    a.work = work;
+    a.sums = (int*)work;
+    a.work = work + ((batch->sessions + 3) & ~3);
     a.qh = q_heads;
     a.kvh = pool->kv_heads;
     a.g = pg_group(q_heads, pool->kv_heads);
@@ -840,7 +921,7 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
                : pool->bits == 8 ? pd_launch<8, 1>(a, st) : pd_launch<4, 1>(a, st);
     if (vecs <= 32)
         return pool->bits == 16 ? pd_launch<16, 2>(a, st)
-               : pool->bits == 8 ? pd_launch<8, 2>(a, st) : pd_launch<4, 2>(a, st);
+               : pool->bits == 8 ? pd_launch<8, 1>(a, st) : pd_launch<4, 1>(a, st);
     const dim3 grid((unsigned)batch->rows, (unsigned)q_heads);
     if (pool->bits == 16) hipLaunchKernelGGL(k_paged_attn<16>, grid, dim3(128), 0, st, a);
     else if (pool->bits == 8) hipLaunchKernelGGL(k_paged_attn<8>, grid, dim3(128), 0, st, a);
