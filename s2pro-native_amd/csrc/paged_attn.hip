@@ -34,80 +34,9 @@ struct PgAttn {
     float* work;
     int* sums; /* [sessions] rounds up to each (the merge's view of the schedule) */
     int qh, kvh, g;
+    int rt; /* rows a tile of k_paged_rows */
     int nb, nvt; /* blocks a kv head that share the rounds, for each tile of query vectors */
 };
-
-template <int BW>
-S2P_DEV float pg_value(const char* row, const uint16_t* sc, int d) {
-    if constexpr (BW == 16) return bf2f(((const uint16_t*)row)[d]);
-    else if constexpr (BW == 8) return (float)((const int8_t*)row)[d] * h2f(sc[d >> 5]);
-    else {
-        const int n = (((const uint8_t*)row)[d >> 1] >> (4 * (d & 1))) & 0xF;
-        return (float)(n >= 8 ? n - 16 : n) * h2f(sc[d >> 5]);
-    }
-}
-
-template <int BW>
-__global__ __launch_bounds__(128) void k_paged_attn(PgAttn a) {
-    constexpr int EL = BW == 16 ? 256 : BW == 8 ? 128 : 64;
-    __shared__ float s_q[128], s_p[128], s_red[2];
-    __shared__ int64_t s_at[128];
-    const int row = blockIdx.x, head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    int s = 0;
-    for (int i = 0; i < a.b.sessions; i += 64)
-        s += __popcll(__ballot(i + lane < a.b.sessions && a.b.row0[i + lane + 1] <= row));
-    if (s >= a.b.sessions) return;
-    const PgSess ss = pg_session(a.b, s);
-    const int i = row - ss.r0;
-    if (i < 0 || i >= ss.n) return;
-    const int kvh = head / a.g;
-    const uint64_t vis = a.vis ? a.vis[row] : 0ull;
-    const int32_t* tab = a.b.table + (size_t)s * a.b.max_pages;
-    s_q[t] = bf2f(a.q[((size_t)row * a.qh + head) * PG_HD + t]) * 0.08838834764831845f;
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    bool any = false;
-    for (int t0 = 0; t0 < ss.L + ss.n; t0 += 128) {
-        const int j = t0 + t, b = j - ss.L;
-        bool seen = j < ss.L + ss.n && (b < 0 || (a.vis ? ((vis >> (b & 63)) & 1) : b <= i));
-        int64_t at = -1;
-        float x = -INFINITY;
-        if (seen) {
-            const int id = tab[j >> a.l.shift];
-            if ((unsigned)id < (unsigned)a.l.pages) {
-                at = (((int64_t)id * a.l.planes + kvh) << a.l.shift) + (j & (a.l.page - 1));
-                const char* k = a.l.kv + at * EL;
-                x = 0.f;
-                for (int d = 0; d < 128; d++)
-                    x = fmaf(s_q[d], pg_value<BW>(k, a.l.sc ? a.l.sc + at * 4 : nullptr, d), x);
-            }
-        }
-        s_at[t] = at;
-        float tm = wave_max(x);
-        if (__syncthreads_or(x != x)) tm = NAN;
-        if (lane == 0) s_red[wave] = tm;
-        any |= __syncthreads_or(at >= 0) != 0;
-        const float mn = fmaxf(m, fmaxf(s_red[0], s_red[1]));
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        const float corr = expf(m - ms);
-        s_p[t] = at >= 0 ? expf(x - ms) : 0.f;
-        __syncthreads();
-        l *= corr;
-        acc *= corr;
-        for (int u = 0; u < 128; u++) {
-            const int64_t v = s_at[u];
-            if (v < 0) continue;
-            const int64_t vat = v + ((int64_t)a.kvh << a.l.shift);
-            l += s_p[u];
-            acc = fmaf(s_p[u],
-                       pg_value<BW>(a.l.kv + vat * EL, a.l.sc ? a.l.sc + vat * 4 : nullptr, t), acc);
-        }
-        m = mn;
-        __syncthreads();
-    }
-    a.out[((size_t)row * a.qh + head) * PG_HD + t] = f2bf(any ? acc / l : 0.f);
-}
-
 
 #define PD_WAVES 4
 #define PD_SCALE (0.08838834764831845f * 1.4426950408889634f) /* log2(e) / sqrt(128) */
@@ -859,6 +788,431 @@ __global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int tile) {
         f2bf(M == -INFINITY && mark == 0.f ? 0.f : z / lt);
 }
 
+/* ------------------------------------------------------------ many rows a session */
+
+#define PR_WAVES 4
+#define PR_VEC (32 * PR_WAVES) /* query vectors of a block: a row tile */
+#define PR_TS 64               /* slots of a tile */
+#define PR_LAZY 8.0f           /* the running maximum follows when p would pass 2^8 */
+
+typedef __attribute__((ext_vector_type(16))) float pr_f32x16;
+S2P_DEV pr_f32x16 mfma32x32x16(s2p_u32x4 a, s2p_u32x4 b, pr_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+/* a K row's 16-byte chunks permuted, and a V row's (for the transposing reads), in elements */
+S2P_DEV int pr_koff(int t, int ch) { return t * PG_HD + ((ch ^ (t & 15)) << 3); }
+S2P_DEV int pr_voff(int t, int ch) { return t * PG_HD + ((ch ^ ((t & 7) << 1)) << 3); }
+S2P_DEV float pr_swap_max(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+S2P_DEV float pr_swap_sum(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+S2P_DEV bool pr_odd(s2p_u32x4 w) { /* eight bf16, one of them NaN or infinite */
+    bool o = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        o |= (w[e] & 0x7F80u) == 0x7F80u || (w[e] & 0x7F800000u) == 0x7F800000u;
+    return o;
+}
+/* tiles of slots that row tile r of a session needs */
+S2P_DEV int pr_rounds(const PgAttn& a, const PgSess& s, int r) {
+    const int span = s.L + (a.vis ? s.n : min(s.n, (r + 1) * a.rt));
+    return (span + PR_TS - 1) / PR_TS;
+}
+
+/* a code pair's element of a word: INT8 word q / 2 of the chunk, INT4 the chunk's one word */
+template <int BW>
+S2P_DEV float pr_code(uint32_t w, int q, int e) {
+    if constexpr (BW == 8) return (float)(int8_t)(w >> (8 * (2 * (q & 1) + e)));
+    else return (float)((int32_t)(w << (28 - 4 * (2 * q + e))) >> 28);
+}
+
+/* what a thread brings of a tile: 16-byte pieces of K and V and their scales */
+template <int BW>
+struct PrStage {
+    static constexpr int EL = BW == 16 ? 256 : BW == 8 ? 128 : 64;
+    static constexpr int NL = PR_TS * EL / (64 * PR_WAVES * 16); /* pieces of each */
+    s2p_u32x4 k[NL], v[NL];
+    uint16_t ks[NL], vs[NL];
+};
+
+template <int BW>
+__global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
+#pragma clang fp contract(off)
+    typedef PrStage<BW> Stage;
+    constexpr int EL = Stage::EL, NL = Stage::NL, CR = EL / 16; /* pieces of a row */
+    __shared__ __align__(256) uint16_t s_k[2][PR_TS * PG_HD], s_v[2][PR_TS * PG_HD];
+    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[PR_WAVES];
+    __shared__ unsigned long long s_odd[2]; /* V rows of nodes with a NaN or infinity */
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5, col = lane & 31;
+    const int kvh = blockIdx.x % a.kvh, blk = blockIdx.x / a.kvh;
+
+    /* the block's share of the rounds of all row tiles */
+    int total = 0;
+    for (int base = 0; base < a.b.sessions; base += 64 * PR_WAVES) {
+        int v = 0;
+        if (base + tid < a.b.sessions) {
+            const PgSess ss = pg_session(a.b, base + tid);
+            for (int r = 0; r * a.rt < ss.n; r++) v += pr_rounds(a, ss, r);
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(v, o, 64);
+            if (lane >= o) v += t;
+        }
+        if (base) __syncthreads();
+        if (lane == 63) s_w[wave] = v;
+        __syncthreads();
+        int all = total;
+#pragma unroll
+        for (int w = 0; w < PR_WAVES; w++) {
+            if (w < wave) v += s_w[w];
+            all += s_w[w];
+        }
+        if (base + tid < a.b.sessions) s_pre[base + tid] = total + v;
+        total = all;
+    }
+    if (tid < 2) s_odd[tid] = 0;
+    __syncthreads();
+    const int nb = min(a.nb, total);
+    if (blk >= nb) {
+        if (kvh == 0 && blk < a.nb && tid == 0) a.sums[4 * blk + 1] = 0;
+        return;
+    }
+    const int begin = (int)((int64_t)blk * total / nb);
+    const int end = (int)((int64_t)(blk + 1) * total / nb);
+
+    const int vec = 32 * wave + col; /* this lane's query vector of a row tile */
+    const int vi = vec / a.g, vhead = kvh * a.g + vec % a.g;
+    int nvec_out = 0; /* of the row tile that the block leaves to another one */
+
+    for (int cur = begin; cur < end;) {
+        int s = 0, hi = a.b.sessions - 1;
+        while (s < hi) {
+            const int mid = (s + hi) >> 1;
+            if (s_pre[mid] > cur) hi = mid;
+            else s = mid + 1;
+        }
+        s = __builtin_amdgcn_readfirstlane(s);
+        const PgSess ss = pg_session(a.b, s);
+        int first = __builtin_amdgcn_readfirstlane(s ? s_pre[s - 1] : 0), r = 0, cnt;
+        while (first + (cnt = pr_rounds(a, ss, r)) <= cur) { /* ends: the session reaches past cur */
+            first += cnt;
+            r++;
+        }
+        const int last = first + cnt, stop = min(end, last);
+        const int i0 = r * a.rt, rows = min(a.rt, ss.n - i0); /* the tile's rows */
+        const int span = ss.L + (a.vis ? ss.n : i0 + rows);   /* slots that one of them may see */
+        const int32_t* tab = a.b.table + (size_t)s * a.b.max_pages;
+        const int nvec = rows * a.g;
+        const bool live = vec < nvec;
+        const bool busy = 32 * wave < nvec; /* the wave has a vector */
+        const int row = ss.r0 + i0 + (live ? vi : 0);
+        /* the row's nodes as a word, or (causal) how many slots it sees */
+        const uint64_t word = a.vis && live ? a.vis[row] & pd_ones(ss.n) : 0ull;
+        const int sees = live ? ss.L + i0 + vi + 1 : 0;
+        /* no row of the wave sees a slot from here on; every one sees those before `open` */
+        const int wend = a.vis ? span : min(span, ss.L + i0 + (min(32 * wave + 31, nvec - 1) / a.g) + 1);
+        const int open_end = a.vis ? ss.L : ss.L + i0 + 32 * wave / a.g + 1;
+
+        s2p_u32x4 qb[8];
+        {
+            const uint16_t* qr = a.q + ((size_t)row * a.qh + (live ? vhead : 0)) * PG_HD + 8 * half;
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++)
+                qb[ks] = live ? *(const s2p_u32x4*)(qr + 16 * ks) : (s2p_u32x4){0u, 0u, 0u, 0u};
+        }
+        float m = -INFINITY, l = 0.f;
+        bool any = false;
+        pr_f32x16 o[4];
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
+
+        const int k0 = cur - first, k1 = stop - first;
+        int ids = 0; /* lane x: the page of the 16-slot group x of 16 tiles, or -1 */
+        auto issue = [&](Stage& t, int k) __attribute__((always_inline)) {
+            if (((k - k0) & 15) == 0) {
+                const int slot = (k + (lane >> 2)) * PR_TS + 16 * (lane & 3);
+                int id = -1;
+                if (slot < span && k + (lane >> 2) < k1) {
+                    id = tab[slot >> a.l.shift];
+                    if ((unsigned)id >= (unsigned)a.l.pages) id = -1;
+                }
+                ids = id;
+            }
+            const uint64_t vplane = (uint64_t)(uint32_t)a.kvh << a.l.shift;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int i = tid + 64 * PR_WAVES * j, trow = i / CR, ch = i % CR;
+                const int g = __builtin_amdgcn_readfirstlane(trow >> 4); /* one group a wave */
+                const int id = max(__builtin_amdgcn_readlane(ids, ((k - k0) & 15) * 4 + g), 0);
+                const uint64_t at =
+                    (((uint64_t)(uint32_t)id * (uint32_t)a.l.planes + (uint32_t)kvh) << a.l.shift) +
+                    (uint32_t)((k * PR_TS + 16 * g) & (a.l.page - 1));
+                const uint32_t off = (uint32_t)((trow & 15) * EL + 16 * ch);
+                t.k[j] = gbl_at<s2p_u32x4>(gbl_base(a.l.kv, at * EL), off);
+                t.v[j] = gbl_at<s2p_u32x4>(gbl_base(a.l.kv, (at + vplane) * EL), off);
+                if constexpr (BW != 16) {
+                    const uint32_t so = (uint32_t)((trow & 15) * 8 + 2 * (BW == 8 ? ch >> 1 : ch));
+                    t.ks[j] = gbl_at<uint16_t>(gbl_base(a.l.sc, at * 8), so);
+                    t.vs[j] = gbl_at<uint16_t>(gbl_base(a.l.sc, (at + vplane) * 8), so);
+                }
+            }
+        };
+        /* groups of tile k that are not there (of the ids at hand) */
+        auto bad_of = [&](int k) __attribute__((always_inline)) {
+            return (int)((__ballot(ids < 0) >> (((k - k0) & 15) * 4)) & 15);
+        };
+        /* tile k to LDS: codes as bf16; V rows that are not there as zeros (what lies there may be
+         * NaN, and 0 x NaN is NaN) */
+        auto store = [&](Stage& t, int k, int buf, int bad) __attribute__((always_inline)) {
+            const bool whole = k * PR_TS + PR_TS <= ss.L && bad == 0;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int i = tid + 64 * PR_WAVES * j, trow = i / CR, ch = i % CR;
+                constexpr int NC = BW == 16 ? 1 : BW == 8 ? 2 : 4; /* 8-dim chunks of a piece */
+                s2p_u32x4 kw[NC], vw[NC];
+                if constexpr (BW == 16) {
+                    kw[0] = t.k[j];
+                    vw[0] = t.v[j];
+                } else {
+                    const float ks = h2f(t.ks[j]), vs = h2f(t.vs[j]);
+#pragma unroll
+                    for (int e = 0; e < NC; e++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const uint32_t wk = BW == 8 ? t.k[j][2 * e + (q >> 1)] : t.k[j][e];
+                            const uint32_t wv = BW == 8 ? t.v[j][2 * e + (q >> 1)] : t.v[j][e];
+                            kw[e][q] = pd_pk(pr_code<BW>(wk, q, 0) * ks, pr_code<BW>(wk, q, 1) * ks);
+                            vw[e][q] = pd_pk(pr_code<BW>(wv, q, 0) * vs, pr_code<BW>(wv, q, 1) * vs);
+                        }
+                }
+                if (!whole) {
+                    const int slot = k * PR_TS + trow;
+                    bool odd = false;
+                    if (slot >= ss.L + ss.n || ((bad >> (trow >> 4)) & 1)) {
+#pragma unroll
+                        for (int e = 0; e < NC; e++) vw[e] = (s2p_u32x4){0u, 0u, 0u, 0u};
+                    } else if (slot >= ss.L) {
+#pragma unroll
+                        for (int e = 0; e < NC; e++) odd |= pr_odd(vw[e]);
+                    }
+                    if (odd) atomicOr(&s_odd[buf], 1ull << trow);
+                }
+#pragma unroll
+                for (int e = 0; e < NC; e++) {
+                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = kw[e];
+                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_v[buf] + pr_voff(trow, NC * ch + e)) = vw[e];
+                }
+            }
+        };
+
+        Stage st;
+        issue(st, k0);
+        int bad = bad_of(k0), next = 0;
+        store(st, k0, 0, bad);
+        if (k0 + 1 < k1) {
+            issue(st, k0 + 1);
+            next = bad_of(k0 + 1);
+        }
+        __syncthreads();
+        for (int k = k0; k < k1; k++) {
+            const int buf = (k - k0) & 1, tb = k * PR_TS;
+            const LDS(uint16_t)* kt = (const LDS(uint16_t)*)s_k[buf];
+            const LDS(uint16_t)* vt = (const LDS(uint16_t)*)s_v[buf];
+            const unsigned long long odd = s_odd[buf];
+            float x[2][16];
+            uint64_t seen = 0;
+            if (busy && tb < wend) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    pr_f32x16 sc;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sc[i] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < 8; ks++)
+                        sc = mfma32x32x16(*(const LDS(s2p_u32x4)*)(kt + pr_koff(32 * h + col, 2 * ks + half)),
+                                          qb[ks], sc);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[h][i] = sc[i];
+                }
+                /* x[h][i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
+                seen = ~0ull;
+                if (tb + PR_TS > open_end || bad) {
+                    seen = (a.vis ? pd_mask(word, ss.L - tb) : pd_ones(max(0, sees - tb))) & pd_groups(bad);
+                    if (!live) seen = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t w = (uint32_t)(seen >> (32 * h)) >> (4 * half);
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (!((w >> (8 * (i >> 2) + (i & 3))) & 1)) x[h][i] = -INFINITY;
+                    }
+                }
+                any |= seen != 0;
+                float tm = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) tm = fmaxf(tm, x[h][i]);
+                tm = pr_swap_max(tm) * PD_SCALE;
+                if (__any(tm > m + PR_LAZY)) {
+                    const float mn = tm > m + PR_LAZY ? tm : m;
+                    const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                    l *= corr;
+#pragma unroll
+                    for (int dt = 0; dt < 4; dt++) o[dt] *= corr;
+                    m = mn;
+                }
+                const float ms = m == -INFINITY ? 0.f : m;
+                float ls = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        x[h][i] = __builtin_amdgcn_exp2f(fmaf(x[h][i], PD_SCALE, -ms));
+                        ls += x[h][i];
+                    }
+                l += ls;
+            }
+            if (odd) { /* uniform: rare */
+                if (busy && tb < wend)
+                    for (unsigned long long w = odd; w; w &= w - 1) {
+                        const int t = __ffsll(w) - 1;
+                        float p = 0.f;
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                p = (t >> 5) == h && ((t >> 3) & 3) == (i >> 2) && (t & 3) == (i & 3)
+                                        ? x[h][i] : p;
+                        p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
+                        if ((seen >> t) & 1) {
+#pragma unroll
+                            for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+                                for (int q = 0; q < 4; q++) {
+                                    const int d = 32 * dt + 8 * q + 4 * half;
+                                    const s2p_u32x2 v =
+                                        *(const LDS(s2p_u32x2)*)(vt + pr_voff(t, d >> 3) + (d & 7));
+                                    o[dt][4 * q] = fmaf(p, bf2f_lo(v.x), o[dt][4 * q]);
+                                    o[dt][4 * q + 1] = fmaf(p, bf2f_hi(v.x), o[dt][4 * q + 1]);
+                                    o[dt][4 * q + 2] = fmaf(p, bf2f_lo(v.y), o[dt][4 * q + 2]);
+                                    o[dt][4 * q + 3] = fmaf(p, bf2f_hi(v.y), o[dt][4 * q + 3]);
+                                }
+                        }
+                    }
+                __syncthreads();
+                for (int i = tid; i < PR_TS * 16; i += 64 * PR_WAVES)
+                    if ((odd >> (i >> 4)) & 1)
+                        *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_v[buf] + i * 8) = (s2p_u32x4){0u, 0u, 0u, 0u};
+                if (tid == 0) s_odd[buf] = 0;
+                __syncthreads();
+            }
+            if (busy && tb < wend) {
+#pragma unroll
+                for (int kb = 0; kb < 4; kb++) {
+                    const float* xs = &x[kb >> 1][8 * (kb & 1)];
+                    const s2p_u32x4 pw = {pd_pk(xs[0], xs[1]), pd_pk(xs[2], xs[3]), pd_pk(xs[4], xs[5]),
+                                          pd_pk(xs[6], xs[7])};
+                    /* rows 16 kb + 4 half + 0 .. 3 and + 8: lane 4 r + c4 gives row r, dims 4 c4 .. */
+                    const int vr = 16 * kb + 4 * half + ((lane >> 2) & 3);
+#pragma unroll
+                    for (int dt = 0; dt < 4; dt++) {
+                        const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                        const s2p_u32x2 b0 = ds_read_tr16(vt + pr_voff(vr, d >> 3) + (d & 7));
+                        const s2p_u32x2 b1 = ds_read_tr16(vt + pr_voff(vr + 8, d >> 3) + (d & 7));
+                        o[dt] = mfma32x32x16((s2p_u32x4){b0.x, b0.y, b1.x, b1.y}, pw, o[dt]);
+                    }
+                }
+            }
+            bad = next;
+            if (k + 1 < k1) {
+                store(st, k + 1, buf ^ 1, bad);
+                if (k + 2 < k1) {
+                    issue(st, k + 2);
+                    next = bad_of(k + 2);
+                }
+            }
+            __syncthreads();
+        }
+        /* out, or the partial of a tile that other blocks work on too */
+        const float lt0 = pr_swap_sum(l);
+        const float lt = m == -INFINITY ? (any ? 1.f : 0.f) : lt0; /* -inf everywhere, not nothing */
+        if (cur == first && stop == last) {
+            const float inv = m == -INFINITY ? (any ? NAN : 0.f) : 1.f / lt;
+            if (live) {
+                uint16_t* out = a.out + ((size_t)row * a.qh + vhead) * PG_HD + 4 * half;
+#pragma unroll
+                for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        *(s2p_u32x2*)(out + 32 * dt + 8 * q) =
+                            (s2p_u32x2){pd_pk(o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv),
+                                        pd_pk(o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv)};
+            }
+        } else {
+            float* const po = a.work + ((size_t)(kvh * a.nb + blk) * 2 + (cur == first ? 1 : 0)) *
+                                           ((size_t)PR_VEC * (PG_HD + 2));
+            if (live) {
+                if (half == 0) {
+                    po[2 * vec] = m;
+                    po[2 * vec + 1] = lt;
+                }
+                float* const pz = po + 2 * PR_VEC + vec * PG_HD + 4 * half;
+#pragma unroll
+                for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        *(s2p_f32x4*)(pz + 32 * dt + 8 * q) =
+                            (s2p_f32x4){o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+            }
+            if (cur == first && kvh == 0 && tid == 0) { /* what begins here and ends elsewhere */
+                a.sums[4 * blk] = ss.r0 + i0;
+                a.sums[4 * blk + 2] = (int)(((int64_t)last * nb - 1) / total); /* its last block */
+            }
+            if (cur == first) nvec_out = nvec;
+        }
+        cur = stop;
+    }
+    if (kvh == 0 && tid == 0) a.sums[4 * blk + 1] = nvec_out;
+}
+
+/* Row tiles that several blocks worked on, from their partials: a block a (block where the tile
+ * begins, kv head, 8 vectors), four dims a thread. */
+__global__ __launch_bounds__(256) void k_paged_rows_merge(PgAttn a) {
+    const int j0 = blockIdx.z, kvh = blockIdx.y;
+    const int vec = blockIdx.x * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+    const int row0 = a.sums[4 * j0], nvec = a.sums[4 * j0 + 1], j1 = a.sums[4 * j0 + 2];
+    if (vec >= nvec) return;
+    const size_t stride = (size_t)PR_VEC * (PG_HD + 2);
+    const float* p = a.work + ((size_t)(kvh * a.nb + j0) * 2 + 1) * stride;
+    float M = p[2 * vec], lt = p[2 * vec + 1], mark = lt;
+    s2p_f32x4 z = *(const s2p_f32x4*)(p + 2 * PR_VEC + vec * PG_HD + d);
+    for (int j = j0 + 1; j <= j1; j++) {
+        p = a.work + (size_t)(kvh * a.nb + j) * 2 * stride;
+        const float pm = p[2 * vec], pl = p[2 * vec + 1];
+        const s2p_f32x4 pz = *(const s2p_f32x4*)(p + 2 * PR_VEC + vec * PG_HD + d);
+        const float mn = fmaxf(M, pm), ms = mn == -INFINITY ? 0.f : mn;
+        const float e0 = __builtin_amdgcn_exp2f(M - ms), e1 = __builtin_amdgcn_exp2f(pm - ms);
+        mark = fmaxf(mark, pl);
+        lt = fmaf(lt, e0, pl * e1);
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e] = fmaf(z[e], e0, pz[e] * e1);
+        M = mn;
+    }
+    const float inv = M == -INFINITY ? (mark > 0.f ? NAN : 0.f) : 1.f / lt;
+    *(s2p_u32x2*)(a.out + ((size_t)(row0 + vec / a.g) * a.qh + kvh * a.g + vec % a.g) * PG_HD + d) =
+        (s2p_u32x2){pd_pk(z[0] * inv, z[1] * inv), pd_pk(z[2] * inv, z[3] * inv)};
+}
+
 /* blocks a kv head and tile of query vectors: as many as fit at once, `each` a CU, and no more
  * than there are rounds of `rnd` slots */
 static int64_t pd_blocks(const s2p_page_batch* b, int tiles, int rnd, int each) {
@@ -883,14 +1237,35 @@ static hipError_t pd_launch(PgAttn a, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <int BW>
+static hipError_t pr_launch(PgAttn a, hipStream_t st) {
+    hipLaunchKernelGGL(k_paged_rows<BW>, dim3((unsigned)(a.nb * a.kvh)), dim3(64 * PR_WAVES), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.nb == 1) return e;
+    hipLaunchKernelGGL(k_paged_rows_merge, dim3(PR_VEC / 8, (unsigned)a.kvh, (unsigned)a.nb), dim3(256),
+                       0, st, a);
+    return hipGetLastError();
+}
+/* blocks a kv head over row tiles: two a CU, no more than there are rounds */
+static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int rt) {
+    const int64_t most = (int64_t)b->sessions * ((b->max_rows + rt - 1) / rt) *
+                         ((b->max_len + PR_TS - 1) / PR_TS);
+    int64_t nb = 2 * s2p_cu_count() / kv_heads;
+    if (nb < 1) nb = 1;
+    return nb < most ? nb : most;
+}
+
 extern "C" int64_t s2pk_paged_attention_work_floats(const s2p_page_batch* batch, int q_heads,
                                                     int kv_heads) {
     if (!batch || batch->sessions <= 0 || batch->rows <= 0 || kv_heads <= 0 ||
         !pg_group(q_heads, kv_heads))
         return 0;
-    const int vecs = batch->max_rows * pg_group(q_heads, kv_heads);
+    const int64_t vecs = (int64_t)batch->max_rows * pg_group(q_heads, kv_heads);
+    if (vecs > 32) {
+        const int64_t nb = pr_blocks(batch, kv_heads, PR_VEC / pg_group(q_heads, kv_heads));
+        return 4 * nb + kv_heads * nb * 2 * PR_VEC * (PG_HD + 2);
+    }
     const int64_t sums = (batch->sessions + 3) & ~3;
-    if (vecs > 32) return sums;
     return sums + kv_heads * pd_blocks(batch, kv_heads, 128, 3) * 2 * (vecs > 16 ? 32 : 16) * (PG_HD + 2);
 }
 
@@ -911,20 +1286,24 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
     a.vis = vis;
     a.out = (uint16_t*)out;
     a.sums = (int*)work;
-    a.work = work + ((batch->sessions + 3) & ~3);
     a.qh = q_heads;
     a.kvh = pool->kv_heads;
     a.g = pg_group(q_heads, pool->kv_heads);
-    const int vecs = batch->max_rows * a.g;
-    if (vecs <= 16)
+    /* rounds are counted in 32 bits */
+    a.rt = PR_VEC / a.g;
+    if ((int64_t)batch->sessions * ((batch->max_rows + a.rt - 1) / a.rt) * ((batch->max_len + 63) / 64) >
+        1 << 30)
+        return hipErrorInvalidValue;
+    const int64_t vecs = (int64_t)batch->max_rows * a.g;
+    if (vecs > 32) {
+        a.nb = (int)pr_blocks(batch, a.kvh, a.rt);
+        a.work = work + 4 * (int64_t)a.nb;
+        return pool->bits == 16 ? pr_launch<16>(a, st)
+               : pool->bits == 8 ? pr_launch<8>(a, st) : pr_launch<4>(a, st);
+    }
+    a.work = work + ((batch->sessions + 3) & ~3);
+    if (vecs <= 16 || pool->bits != 16)
         return pool->bits == 16 ? pd_launch<16, 1>(a, st)
                : pool->bits == 8 ? pd_launch<8, 1>(a, st) : pd_launch<4, 1>(a, st);
-    if (vecs <= 32)
-        return pool->bits == 16 ? pd_launch<16, 2>(a, st)
-               : pool->bits == 8 ? pd_launch<8, 1>(a, st) : pd_launch<4, 1>(a, st);
-    const dim3 grid((unsigned)batch->rows, (unsigned)q_heads);
-    if (pool->bits == 16) hipLaunchKernelGGL(k_paged_attn<16>, grid, dim3(128), 0, st, a);
-    else if (pool->bits == 8) hipLaunchKernelGGL(k_paged_attn<8>, grid, dim3(128), 0, st, a);
-    else hipLaunchKernelGGL(k_paged_attn<4>, grid, dim3(128), 0, st, a);
-    return hipGetLastError();
+    return pd_launch<16, 2>(a, st);
 }
