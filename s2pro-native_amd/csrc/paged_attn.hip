@@ -790,14 +790,22 @@ __global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int tile) {
 
 /* ------------------------------------------------------------ many rows a session */
 
-#define PR_WAVES 4
-#define PR_VEC (32 * PR_WAVES) /* query vectors of a block: a row tile */
 #define PR_TS 64               /* slots of a tile */
 #define PR_LAZY 8.0f           /* the running maximum follows when p would pass 2^8 */
 
 typedef __attribute__((ext_vector_type(16))) float pr_f32x16;
 S2P_DEV pr_f32x16 mfma32x32x16(s2p_u32x4 a, s2p_u32x4 b, pr_f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+S2P_DEV pr_f32x16 mfma32x32x16_f16(s2p_u32x4 a, s2p_u32x4 b, pr_f32x16 c) {
+    typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+S2P_DEV uint32_t pr_pk_f16(float a, float b) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f2;
+    typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 h2;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
 }
 /* a K row's 16-byte chunks permuted, and a V row's (for the transposing reads), in elements */
 S2P_DEV int pr_koff(int t, int ch) { return t * PG_HD + ((ch ^ (t & 15)) << 3); }
@@ -830,23 +838,27 @@ S2P_DEV float pr_code(uint32_t w, int q, int e) {
     else return (float)((int32_t)(w << (28 - 4 * (2 * q + e))) >> 28);
 }
 
-/* what a thread brings of a tile: 16-byte pieces of K and V and their scales */
-template <int BW>
+/* what a thread brings of a tile's K or V: 16-byte pieces and their scales */
+template <int BW, int W>
 struct PrStage {
     static constexpr int EL = BW == 16 ? 256 : BW == 8 ? 128 : 64;
-    static constexpr int NL = PR_TS * EL / (64 * PR_WAVES * 16); /* pieces of each */
-    s2p_u32x4 k[NL], v[NL];
-    uint16_t ks[NL], vs[NL];
+    static constexpr int NP = PR_TS * EL / 16;                       /* pieces of a tile's K or V */
+    static constexpr int NL = (NP + 64 * W - 1) / (64 * W);
+    s2p_u32x4 w[NL];
+    uint16_t s[NL];
 };
 
-template <int BW>
-__global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
+template <int BW, int W>
+__global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
 #pragma clang fp contract(off)
-    typedef PrStage<BW> Stage;
+    typedef PrStage<BW, W> Stage;
+    constexpr int VEC = 32 * W; /* query vectors of a row tile */
     constexpr int EL = Stage::EL, NL = Stage::NL, CR = EL / 16; /* pieces of a row */
+    constexpr int NC = BW == 16 ? 1 : BW == 8 ? 2 : 4;         /* 8-dim chunks of a piece */
     __shared__ __align__(256) uint16_t s_k[2][PR_TS * PG_HD], s_v[2][PR_TS * PG_HD];
-    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[PR_WAVES];
-    __shared__ unsigned long long s_odd[2]; /* V rows of nodes with a NaN or infinity */
+    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[W];
+    __shared__ unsigned long long s_odd[3]; /* bf16: nodes whose V holds a NaN or infinity */
+    __shared__ __align__(16) uint16_t s_vs[BW == 16 ? 1 : 2][PR_TS][4]; /* codes: V scales */
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, col = lane & 31;
@@ -854,7 +866,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
 
     /* the block's share of the rounds of all row tiles */
     int total = 0;
-    for (int base = 0; base < a.b.sessions; base += 64 * PR_WAVES) {
+    for (int base = 0; base < a.b.sessions; base += 64 * W) {
         int v = 0;
         if (base + tid < a.b.sessions) {
             const PgSess ss = pg_session(a.b, base + tid);
@@ -870,14 +882,14 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
         __syncthreads();
         int all = total;
 #pragma unroll
-        for (int w = 0; w < PR_WAVES; w++) {
+        for (int w = 0; w < W; w++) {
             if (w < wave) v += s_w[w];
             all += s_w[w];
         }
         if (base + tid < a.b.sessions) s_pre[base + tid] = total + v;
         total = all;
     }
-    if (tid < 2) s_odd[tid] = 0;
+    if (tid < 3) s_odd[tid] = 0;
     __syncthreads();
     const int nb = min(a.nb, total);
     if (blk >= nb) {
@@ -890,6 +902,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
     const int vec = 32 * wave + col; /* this lane's query vector of a row tile */
     const int vi = vec / a.g, vhead = kvh * a.g + vec % a.g;
     int nvec_out = 0; /* of the row tile that the block leaves to another one */
+    int seq = 0;      /* tiles so far, mod 3 */
 
     for (int cur = begin; cur < end;) {
         int s = 0, hi = a.b.sessions - 1;
@@ -921,11 +934,31 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
         const int open_end = a.vis ? ss.L : ss.L + i0 + 32 * wave / a.g + 1;
 
         s2p_u32x4 qb[8];
+        float scale = PD_SCALE;
         {
             const uint16_t* qr = a.q + ((size_t)row * a.qh + (live ? vhead : 0)) * PG_HD + 8 * half;
 #pragma unroll
             for (int ks = 0; ks < 8; ks++)
                 qb[ks] = live ? *(const s2p_u32x4*)(qr + 16 * ks) : (s2p_u32x4){0u, 0u, 0u, 0u};
+            if constexpr (BW != 16) {
+                /* q in f16: exact (11 bits for 8) below 2^15, larger vectors as multiples of a
+                 * power of two; the power, and K's 2^-7, go into the scale */
+                uint32_t top = 0;
+#pragma unroll
+                for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        top = max(top, max(qb[ks][e] & 0x7FFFu, (qb[ks][e] >> 16) & 0x7FFFu));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+                const int up = min(max((int)(top >> 7) - (127 + 14), 0), 112);
+                const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+                scale *= __uint_as_float((uint32_t)(127 + 7) << 23) * __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+                for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        qb[ks][e] = pr_pk_f16(bf2f_lo(qb[ks][e]) * down, bf2f_hi(qb[ks][e]) * down);
+            }
         }
         float m = -INFINITY, l = 0.f;
         bool any = false;
@@ -937,7 +970,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
 
         const int k0 = cur - first, k1 = stop - first;
         int ids = 0; /* lane x: the page of the 16-slot group x of 16 tiles, or -1 */
-        auto issue = [&](Stage& t, int k) __attribute__((always_inline)) {
+        auto page_ids = [&](int k) __attribute__((always_inline)) {
             if (((k - k0) & 15) == 0) {
                 const int slot = (k + (lane >> 2)) * PR_TS + 16 * (lane & 3);
                 int id = -1;
@@ -947,79 +980,95 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
                 }
                 ids = id;
             }
-            const uint64_t vplane = (uint64_t)(uint32_t)a.kvh << a.l.shift;
+        };
+        /* tile k's K (is_v: V) into registers */
+        auto issue = [&](Stage& t, int k, bool is_v) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int i = tid + 64 * PR_WAVES * j, trow = i / CR, ch = i % CR;
+                const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
+                if (Stage::NP % (64 * W) && i >= Stage::NP) break; /* whole waves */
                 const int g = __builtin_amdgcn_readfirstlane(trow >> 4); /* one group a wave */
                 const int id = max(__builtin_amdgcn_readlane(ids, ((k - k0) & 15) * 4 + g), 0);
-                const uint64_t at =
-                    (((uint64_t)(uint32_t)id * (uint32_t)a.l.planes + (uint32_t)kvh) << a.l.shift) +
-                    (uint32_t)((k * PR_TS + 16 * g) & (a.l.page - 1));
-                const uint32_t off = (uint32_t)((trow & 15) * EL + 16 * ch);
-                t.k[j] = gbl_at<s2p_u32x4>(gbl_base(a.l.kv, at * EL), off);
-                t.v[j] = gbl_at<s2p_u32x4>(gbl_base(a.l.kv, (at + vplane) * EL), off);
-                if constexpr (BW != 16) {
-                    const uint32_t so = (uint32_t)((trow & 15) * 8 + 2 * (BW == 8 ? ch >> 1 : ch));
-                    t.ks[j] = gbl_at<uint16_t>(gbl_base(a.l.sc, at * 8), so);
-                    t.vs[j] = gbl_at<uint16_t>(gbl_base(a.l.sc, (at + vplane) * 8), so);
-                }
+                const uint64_t at = (((uint64_t)(uint32_t)id * (uint32_t)a.l.planes +
+                                      (uint32_t)(is_v ? a.kvh + kvh : kvh)) << a.l.shift) +
+                                    (uint32_t)((k * PR_TS + 16 * g) & (a.l.page - 1));
+                t.w[j] = gbl_at<s2p_u32x4>(gbl_base(a.l.kv, at * EL), (uint32_t)((trow & 15) * EL + 16 * ch));
+                if constexpr (BW != 16)
+                    t.s[j] = gbl_at<uint16_t>(gbl_base(a.l.sc, at * 8),
+                                              (uint32_t)((trow & 15) * 8 + 2 * (BW == 8 ? ch >> 1 : ch)));
             }
         };
         /* groups of tile k that are not there (of the ids at hand) */
         auto bad_of = [&](int k) __attribute__((always_inline)) {
             return (int)((__ballot(ids < 0) >> (((k - k0) & 15) * 4)) & 15);
         };
-        /* tile k to LDS: codes as bf16; V rows that are not there as zeros (what lies there may be
-         * NaN, and 0 x NaN is NaN) */
-        auto store = [&](Stage& t, int k, int buf, int bad) __attribute__((always_inline)) {
+        /* tile k to LDS.  Codes: K x scale x 2^-7 in f16 (never past its range, 2^-12 off), V's codes
+         * in bf16 (exact) and their scales.  bf16: V rows that are not there become zeros (what
+         * lies there may be NaN, and 0 x NaN is NaN), and so do pieces of a node's V with a NaN or
+         * infinity, which the rows that see the node add by themselves. */
+        auto store_k = [&](Stage& t, int buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
+                if (Stage::NP % (64 * W) && i >= Stage::NP) break;
+                const float ks = BW == 16 ? 1.f : h2f(t.s[j]) * 0.0078125f;
+#pragma unroll
+                for (int e = 0; e < NC; e++) {
+                    s2p_u32x4 w = t.w[j];
+                    if constexpr (BW != 16) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const uint32_t x = BW == 8 ? t.w[j][2 * e + (q >> 1)] : t.w[j][e];
+                            w[q] = pr_pk_f16(pr_code<BW>(x, q, 0) * ks, pr_code<BW>(x, q, 1) * ks);
+                        }
+                    }
+                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = w;
+                }
+            }
+        };
+        auto store_v = [&](Stage& t, int k, int buf, int bad, int slot3) __attribute__((always_inline)) {
             const bool whole = k * PR_TS + PR_TS <= ss.L && bad == 0;
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int i = tid + 64 * PR_WAVES * j, trow = i / CR, ch = i % CR;
-                constexpr int NC = BW == 16 ? 1 : BW == 8 ? 2 : 4; /* 8-dim chunks of a piece */
-                s2p_u32x4 kw[NC], vw[NC];
+                const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
+                if (Stage::NP % (64 * W) && i >= Stage::NP) break;
                 if constexpr (BW == 16) {
-                    kw[0] = t.k[j];
-                    vw[0] = t.v[j];
-                } else {
-                    const float ks = h2f(t.ks[j]), vs = h2f(t.vs[j]);
-#pragma unroll
-                    for (int e = 0; e < NC; e++)
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint32_t wk = BW == 8 ? t.k[j][2 * e + (q >> 1)] : t.k[j][e];
-                            const uint32_t wv = BW == 8 ? t.v[j][2 * e + (q >> 1)] : t.v[j][e];
-                            kw[e][q] = pd_pk(pr_code<BW>(wk, q, 0) * ks, pr_code<BW>(wk, q, 1) * ks);
-                            vw[e][q] = pd_pk(pr_code<BW>(wv, q, 0) * vs, pr_code<BW>(wv, q, 1) * vs);
-                        }
-                }
-                if (!whole) {
-                    const int slot = k * PR_TS + trow;
-                    bool odd = false;
-                    if (slot >= ss.L + ss.n || ((bad >> (trow >> 4)) & 1)) {
-#pragma unroll
-                        for (int e = 0; e < NC; e++) vw[e] = (s2p_u32x4){0u, 0u, 0u, 0u};
-                    } else if (slot >= ss.L) {
-#pragma unroll
-                        for (int e = 0; e < NC; e++) odd |= pr_odd(vw[e]);
+                    if (!whole) {
+                        const int slot = k * PR_TS + trow;
+                        const bool gone = slot >= ss.L + ss.n || ((bad >> (trow >> 4)) & 1);
+                        const bool odd = !gone && slot >= ss.L && pr_odd(t.w[j]);
+                        if (gone || odd) t.w[j] = (s2p_u32x4){0u, 0u, 0u, 0u};
+                        if (odd) atomicOr(&s_odd[slot3], 1ull << trow);
                     }
-                    if (odd) atomicOr(&s_odd[buf], 1ull << trow);
+                } else {
+                    if (BW == 4 || !(ch & 1)) s_vs[buf][trow][BW == 4 ? ch : ch >> 1] = t.s[j];
                 }
 #pragma unroll
                 for (int e = 0; e < NC; e++) {
-                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = kw[e];
-                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_v[buf] + pr_voff(trow, NC * ch + e)) = vw[e];
+                    s2p_u32x4 w = t.w[j];
+                    if constexpr (BW != 16) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const uint32_t x = BW == 8 ? t.w[j][2 * e + (q >> 1)] : t.w[j][e];
+                            w[q] = pd_pk(pr_code<BW>(x, q, 0), pr_code<BW>(x, q, 1));
+                        }
+                    }
+                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_v[buf] + pr_voff(trow, NC * ch + e)) = w;
                 }
             }
         };
 
-        Stage st;
-        issue(st, k0);
+        /* the next tile is on its way while one is worked on */
+        Stage sk, sv;
+        page_ids(k0);
+        issue(sk, k0, false);
+        issue(sv, k0, true);
         int bad = bad_of(k0), next = 0;
-        store(st, k0, 0, bad);
+        store_k(sk, 0);
+        store_v(sv, k0, 0, bad, seq);
         if (k0 + 1 < k1) {
-            issue(st, k0 + 1);
+            issue(sk, k0 + 1, false);
+            issue(sv, k0 + 1, true);
             next = bad_of(k0 + 1);
         }
         __syncthreads();
@@ -1027,42 +1076,80 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
             const int buf = (k - k0) & 1, tb = k * PR_TS;
             const LDS(uint16_t)* kt = (const LDS(uint16_t)*)s_k[buf];
             const LDS(uint16_t)* vt = (const LDS(uint16_t)*)s_v[buf];
-            const unsigned long long odd = s_odd[buf];
-            float x[2][16];
-            uint64_t seen = 0;
-            if (busy && tb < wend) {
+            const int after = seq == 2 ? 0 : seq + 1;
+            unsigned long long odd = 0;
+            if constexpr (BW == 16) {
+                odd = s_odd[seq];
+                if (tid == 0) s_odd[seq ? seq - 1 : 2] = 0; /* everybody has read it, nobody set it again */
+            }
+            const bool work = busy && tb < wend;
+            const bool open = tb + PR_TS <= open_end && bad == 0;
+            uint64_t seen = ~0ull;
+            if (!open) {
+                seen = (a.vis ? pd_mask(word, ss.L - tb) : pd_ones(max(0, sees - tb))) & pd_groups(bad);
+                if (!live) seen = 0;
+            }
+            any |= work && seen != 0;
+            /* byte addresses in LDS: the permuted chunk is the row's own, xor the operand's number
+             * (made here for every tile: kept, they would cost a register a read) */
+            uint32_t ka = pd_lds((const LDS(unsigned char)*)kt) + col * 256 + ((half ^ (col & 15)) << 4);
+            uint32_t va;
+            {
+                const int r = 4 * half + ((lane >> 2) & 3);
+                va = pd_lds((const LDS(unsigned char)*)vt) + r * 256 +
+                     (((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ (r << 1)) << 4) + 8 * (lane & 1);
+            }
+            asm volatile("" : "+v"(ka), "+v"(va));
+            s2p_u32x4 kr[8];
+            auto read_k = [&](int h) __attribute__((always_inline)) { /* slots 32 h + col */
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    pr_f32x16 sc;
+                for (int ks = 0; ks < 8; ks++)
+                    kr[ks] = *(const LDS(s2p_u32x4)*)((const LDS(unsigned char)*)(uintptr_t)(ka ^ (ks << 5)) +
+                                                      8192 * h);
+                __builtin_amdgcn_sched_barrier(0); /* the reads are out before what follows */
+            };
+            /* V^T operand of dims 32 dt .., slots 16 kb + 4 half + 0 .. 3 and + 8: lane 4 r + c
+             * gives row r, dims 4 c .. */
+            auto read_v = [&](int kb, int dt) __attribute__((always_inline)) {
+                const LDS(unsigned char)* p =
+                    (const LDS(unsigned char)*)(uintptr_t)(va ^ (dt << 6)) + 4096 * kb;
+                const s2p_u32x2 b0 = ds_read_tr16((const LDS(uint16_t)*)p);
+                const s2p_u32x2 b1 = ds_read_tr16((const LDS(uint16_t)*)(p + 2048));
+                return (s2p_u32x4){b0.x, b0.y, b1.x, b1.y};
+            };
+            if (work) read_k(0);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) sc[i] = 0.f;
+            for (int h = 0; h < 2; h++) { /* halves of 32 slots */
+              if (work) {
+                pr_f32x16 sc;
 #pragma unroll
-                    for (int ks = 0; ks < 8; ks++)
-                        sc = mfma32x32x16(*(const LDS(s2p_u32x4)*)(kt + pr_koff(32 * h + col, 2 * ks + half)),
-                                          qb[ks], sc);
+                for (int i = 0; i < 16; i++) sc[i] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) x[h][i] = sc[i];
+                for (int ks = 0; ks < 8; ks++)
+                    sc = BW == 16 ? mfma32x32x16(kr[ks], qb[ks], sc) : mfma32x32x16_f16(kr[ks], qb[ks], sc);
+                __builtin_amdgcn_sched_barrier(0);
+                /* the next operands are read while the softmax runs */
+                s2p_u32x4 vr[2][4];
+                if constexpr (BW == 16) {
+#pragma unroll
+                    for (int dt = 0; dt < 4; dt++) vr[0][dt] = read_v(2 * h, dt);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                /* x[h][i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
-                seen = ~0ull;
-                if (tb + PR_TS > open_end || bad) {
-                    seen = (a.vis ? pd_mask(word, ss.L - tb) : pd_ones(max(0, sees - tb))) & pd_groups(bad);
-                    if (!live) seen = 0;
+                if (h == 0) read_k(1);
+                /* x[i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
+                float x[16];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t w = (uint32_t)(seen >> (32 * h)) >> (4 * half);
+                for (int i = 0; i < 16; i++) x[i] = sc[i];
+                const uint32_t mine = (uint32_t)(seen >> (32 * h)) >> (4 * half);
+                if (!open) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (!((w >> (8 * (i >> 2) + (i & 3))) & 1)) x[h][i] = -INFINITY;
-                    }
+                    for (int i = 0; i < 16; i++)
+                        if (!((mine >> (8 * (i >> 2) + (i & 3))) & 1)) x[i] = -INFINITY;
                 }
-                any |= seen != 0;
-                float tm = -INFINITY;
+                float tm = x[0];
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) tm = fmaxf(tm, x[h][i]);
-                tm = pr_swap_max(tm) * PD_SCALE;
+                for (int i = 1; i < 16; i++) tm = fmaxf(tm, x[i]);
+                tm = pr_swap_max(tm) * scale;
                 if (__any(tm > m + PR_LAZY)) {
                     const float mn = tm > m + PR_LAZY ? tm : m;
                     const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -1074,73 +1161,96 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
                 const float ms = m == -INFINITY ? 0.f : m;
                 float ls = 0.f;
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        x[h][i] = __builtin_amdgcn_exp2f(fmaf(x[h][i], PD_SCALE, -ms));
-                        ls += x[h][i];
-                    }
+                for (int i = 0; i < 16; i++) {
+                    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale, -ms));
+                    ls += x[i];
+                }
                 l += ls;
-            }
-            if (odd) { /* uniform: rare */
-                if (busy && tb < wend)
-                    for (unsigned long long w = odd; w; w &= w - 1) {
-                        const int t = __ffsll(w) - 1;
-                        float p = 0.f;
-#pragma unroll
-                        for (int h = 0; h < 2; h++)
+                if constexpr (BW == 16) {
+                    if (odd) { /* uniform and rare: what store() left out, from the page itself */
+                        for (uint32_t w = (uint32_t)(odd >> (32 * h)); w; w &= w - 1) {
+                            const int t = __ffs(w) - 1, slot = tb + 32 * h + t;
+                            float p = 0.f;
 #pragma unroll
                             for (int i = 0; i < 16; i++)
-                                p = (t >> 5) == h && ((t >> 3) & 3) == (i >> 2) && (t & 3) == (i & 3)
-                                        ? x[h][i] : p;
-                        p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
-                        if ((seen >> t) & 1) {
+                                p = (t >> 3) == (i >> 2) && (t & 3) == (i & 3) ? x[i] : p;
+                            p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
+                            if ((seen >> (32 * h + t)) & 1) {
+                                const int id = tab[slot >> a.l.shift]; /* there: its bit is set */
+                                const char* vp = a.l.kv +
+                                    ((((size_t)id * a.l.planes + a.kvh + kvh) << a.l.shift) +
+                                     (slot & (a.l.page - 1))) * EL;
 #pragma unroll
-                            for (int dt = 0; dt < 4; dt++)
+                                for (int i = 0; i < 16; i++) { /* o[i / 4], dims 8 (i % 4) + 4 half .. */
+                                    const s2p_u32x4 w8 = *(const s2p_u32x4*)(vp + 64 * (i >> 2) + 16 * (i & 3));
+                                    if (!pr_odd(w8)) continue;
 #pragma unroll
-                                for (int q = 0; q < 4; q++) {
-                                    const int d = 32 * dt + 8 * q + 4 * half;
-                                    const s2p_u32x2 v =
-                                        *(const LDS(s2p_u32x2)*)(vt + pr_voff(t, d >> 3) + (d & 7));
-                                    o[dt][4 * q] = fmaf(p, bf2f_lo(v.x), o[dt][4 * q]);
-                                    o[dt][4 * q + 1] = fmaf(p, bf2f_hi(v.x), o[dt][4 * q + 1]);
-                                    o[dt][4 * q + 2] = fmaf(p, bf2f_lo(v.y), o[dt][4 * q + 2]);
-                                    o[dt][4 * q + 3] = fmaf(p, bf2f_hi(v.y), o[dt][4 * q + 3]);
+                                    for (int e = 0; e < 4; e++) {
+                                        const uint32_t d = half ? w8[2 + (e >> 1)] : w8[e >> 1];
+                                        o[i >> 2][4 * (i & 3) + e] =
+                                            fmaf(p, e & 1 ? bf2f_hi(d) : bf2f_lo(d), o[i >> 2][4 * (i & 3) + e]);
+                                    }
                                 }
+                            }
                         }
                     }
-                __syncthreads();
-                for (int i = tid; i < PR_TS * 16; i += 64 * PR_WAVES)
-                    if ((odd >> (i >> 4)) & 1)
-                        *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_v[buf] + i * 8) = (s2p_u32x4){0u, 0u, 0u, 0u};
-                if (tid == 0) s_odd[buf] = 0;
-                __syncthreads();
-            }
-            if (busy && tb < wend) {
 #pragma unroll
-                for (int kb = 0; kb < 4; kb++) {
-                    const float* xs = &x[kb >> 1][8 * (kb & 1)];
-                    const s2p_u32x4 pw = {pd_pk(xs[0], xs[1]), pd_pk(xs[2], xs[3]), pd_pk(xs[4], xs[5]),
-                                          pd_pk(xs[6], xs[7])};
-                    /* rows 16 kb + 4 half + 0 .. 3 and + 8: lane 4 r + c4 gives row r, dims 4 c4 .. */
-                    const int vr = 16 * kb + 4 * half + ((lane >> 2) & 3);
+                    for (int dt = 0; dt < 4; dt++) vr[1][dt] = read_v(2 * h + 1, dt);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int dt = 0; dt < 4; dt++) {
-                        const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                        const s2p_u32x2 b0 = ds_read_tr16(vt + pr_voff(vr, d >> 3) + (d & 7));
-                        const s2p_u32x2 b1 = ds_read_tr16(vt + pr_voff(vr + 8, d >> 3) + (d & 7));
-                        o[dt] = mfma32x32x16((s2p_u32x4){b0.x, b0.y, b1.x, b1.y}, pw, o[dt]);
+                    for (int b = 0; b < 2; b++) {
+                        const s2p_u32x4 pw = {pd_pk(x[8 * b], x[8 * b + 1]), pd_pk(x[8 * b + 2], x[8 * b + 3]),
+                                              pd_pk(x[8 * b + 4], x[8 * b + 5]), pd_pk(x[8 * b + 6], x[8 * b + 7])};
+#pragma unroll
+                        for (int dt = 0; dt < 4; dt++) o[dt] = mfma32x32x16(vr[b][dt], pw, o[dt]);
+                    }
+                } else {
+                    /* a scale group is a tile of 32 dims: p times the group's scale is its weight */
+#pragma unroll
+                    for (int gp = 0; gp < 2; gp++) {
+                        uint32_t vs[16]; /* scales of groups 2 gp, 2 gp + 1 of x[i]'s slot */
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            vs[i] = *(const LDS(uint32_t)*)((const LDS(uint16_t)*)&s_vs[buf][0][0] +
+                                                            4 * (32 * h + 8 * (i >> 2) + 4 * half + (i & 3)) + 2 * gp);
+#pragma unroll
+                        for (int g = 0; g < 2; g++) {
+                            const int dt = 2 * gp + g;
+                            s2p_u32x4 va[2];
+#pragma unroll
+                            for (int b = 0; b < 2; b++) va[b] = read_v(2 * h + b, dt);
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int b = 0; b < 2; b++) {
+                                s2p_u32x4 pw;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const int i = 8 * b + 2 * e;
+                                    pw[e] = pd_pk(fmaf(pd_half(vs[i], g), x[i], 0.f),
+                                                  fmaf(pd_half(vs[i + 1], g), x[i + 1], 0.f));
+                                    if (!open) /* a scale may be NaN where the slot is not seen */
+                                        pw[e] &= ((mine >> (8 * (i >> 2) + (i & 3))) & 1 ? 0xFFFFu : 0u) |
+                                                 ((mine >> (8 * (i >> 2) + (i & 3) + 1)) & 1 ? 0xFFFF0000u : 0u);
+                                }
+                                o[dt] = mfma32x32x16(va[b], pw, o[dt]);
+                            }
+                        }
                     }
                 }
+              }
             }
             bad = next;
             if (k + 1 < k1) {
-                store(st, k + 1, buf ^ 1, bad);
+                store_k(sk, buf ^ 1);
+                store_v(sv, k + 1, buf ^ 1, bad, after);
                 if (k + 2 < k1) {
-                    issue(st, k + 2);
+                    page_ids(k + 2);
+                    issue(sk, k + 2, false);
+                    issue(sv, k + 2, true);
                     next = bad_of(k + 2);
                 }
             }
+            seq = after;
             __syncthreads();
         }
         /* out, or the partial of a tile that other blocks work on too */
@@ -1160,13 +1270,13 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
             }
         } else {
             float* const po = a.work + ((size_t)(kvh * a.nb + blk) * 2 + (cur == first ? 1 : 0)) *
-                                           ((size_t)PR_VEC * (PG_HD + 2));
+                                           ((size_t)VEC * (PG_HD + 2));
             if (live) {
                 if (half == 0) {
                     po[2 * vec] = m;
                     po[2 * vec + 1] = lt;
                 }
-                float* const pz = po + 2 * PR_VEC + vec * PG_HD + 4 * half;
+                float* const pz = po + 2 * VEC + vec * PG_HD + 4 * half;
 #pragma unroll
                 for (int dt = 0; dt < 4; dt++)
 #pragma unroll
@@ -1187,19 +1297,19 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void k_paged_rows(PgAttn a) {
 
 /* Row tiles that several blocks worked on, from their partials: a block a (block where the tile
  * begins, kv head, 8 vectors), four dims a thread. */
-__global__ __launch_bounds__(256) void k_paged_rows_merge(PgAttn a) {
+__global__ __launch_bounds__(256) void k_paged_rows_merge(PgAttn a, int tile) {
     const int j0 = blockIdx.z, kvh = blockIdx.y;
     const int vec = blockIdx.x * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
     const int row0 = a.sums[4 * j0], nvec = a.sums[4 * j0 + 1], j1 = a.sums[4 * j0 + 2];
     if (vec >= nvec) return;
-    const size_t stride = (size_t)PR_VEC * (PG_HD + 2);
+    const size_t stride = (size_t)tile * (PG_HD + 2);
     const float* p = a.work + ((size_t)(kvh * a.nb + j0) * 2 + 1) * stride;
     float M = p[2 * vec], lt = p[2 * vec + 1], mark = lt;
-    s2p_f32x4 z = *(const s2p_f32x4*)(p + 2 * PR_VEC + vec * PG_HD + d);
+    s2p_f32x4 z = *(const s2p_f32x4*)(p + 2 * tile + vec * PG_HD + d);
     for (int j = j0 + 1; j <= j1; j++) {
         p = a.work + (size_t)(kvh * a.nb + j) * 2 * stride;
         const float pm = p[2 * vec], pl = p[2 * vec + 1];
-        const s2p_f32x4 pz = *(const s2p_f32x4*)(p + 2 * PR_VEC + vec * PG_HD + d);
+        const s2p_f32x4 pz = *(const s2p_f32x4*)(p + 2 * tile + vec * PG_HD + d);
         const float mn = fmaxf(M, pm), ms = mn == -INFINITY ? 0.f : mn;
         const float e0 = __builtin_amdgcn_exp2f(M - ms), e1 = __builtin_amdgcn_exp2f(pm - ms);
         mark = fmaxf(mark, pl);
@@ -1237,20 +1347,26 @@ static hipError_t pd_launch(PgAttn a, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <int BW>
+template <int BW, int W>
 static hipError_t pr_launch(PgAttn a, hipStream_t st) {
-    hipLaunchKernelGGL(k_paged_rows<BW>, dim3((unsigned)(a.nb * a.kvh)), dim3(64 * PR_WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_paged_rows<BW, W>), dim3((unsigned)(a.nb * a.kvh)), dim3(64 * W), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nb == 1) return e;
-    hipLaunchKernelGGL(k_paged_rows_merge, dim3(PR_VEC / 8, (unsigned)a.kvh, (unsigned)a.nb), dim3(256),
-                       0, st, a);
+    hipLaunchKernelGGL(k_paged_rows_merge, dim3(4 * W, (unsigned)a.kvh, (unsigned)a.nb), dim3(256), 0,
+                       st, a, 32 * W);
     return hipGetLastError();
 }
-/* blocks a kv head over row tiles: two a CU, no more than there are rounds */
-static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int rt) {
+/* Waves of a block.  Eight read K and V half as often as four and have registers for the next
+ * tile: 2 x 2,048 bf16 rows take 240 us, 300 in fours; four 17-row trees at 8,192 tokens 48 and 52.
+ * Over codes four (two blocks a CU) for up to 128 query vectors, where the conversion would wait
+ * for three waves' work: the trees take 58 us over INT4 codes, 72 in eights. */
+static int pr_waves(int64_t vecs, bool codes) { return codes && vecs <= 128 ? 4 : 8; }
+/* blocks a kv head over row tiles: eight waves a CU, no more than there are rounds */
+static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int g, int w) {
+    const int rt = 32 * w / g;
     const int64_t most = (int64_t)b->sessions * ((b->max_rows + rt - 1) / rt) *
                          ((b->max_len + PR_TS - 1) / PR_TS);
-    int64_t nb = 2 * s2p_cu_count() / kv_heads;
+    int64_t nb = 8 / w * s2p_cu_count() / kv_heads;
     if (nb < 1) nb = 1;
     return nb < most ? nb : most;
 }
@@ -1262,8 +1378,14 @@ extern "C" int64_t s2pk_paged_attention_work_floats(const s2p_page_batch* batch,
         return 0;
     const int64_t vecs = (int64_t)batch->max_rows * pg_group(q_heads, kv_heads);
     if (vecs > 32) {
-        const int64_t nb = pr_blocks(batch, kv_heads, PR_VEC / pg_group(q_heads, kv_heads));
-        return 4 * nb + kv_heads * nb * 2 * PR_VEC * (PG_HD + 2);
+        const int g = pg_group(q_heads, kv_heads);
+        int64_t most = 0; /* either kind of cache */
+        for (int w = 4; w <= 8; w += 4) {
+            const int64_t nb = pr_blocks(batch, kv_heads, g, w);
+            const int64_t n = 4 * nb + kv_heads * nb * 2 * 32 * w * (PG_HD + 2);
+            if (n > most) most = n;
+        }
+        return most;
     }
     const int64_t sums = (batch->sessions + 3) & ~3;
     return sums + kv_heads * pd_blocks(batch, kv_heads, 128, 3) * 2 * (vecs > 16 ? 32 : 16) * (PG_HD + 2);
@@ -1289,17 +1411,19 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
     a.qh = q_heads;
     a.kvh = pool->kv_heads;
     a.g = pg_group(q_heads, pool->kv_heads);
+    const int64_t vecs = (int64_t)batch->max_rows * a.g;
+    const int w = pr_waves(vecs, pool->bits != 16);
+    a.rt = 32 * w / a.g;
     /* rounds are counted in 32 bits */
-    a.rt = PR_VEC / a.g;
     if ((int64_t)batch->sessions * ((batch->max_rows + a.rt - 1) / a.rt) * ((batch->max_len + 63) / 64) >
         1 << 30)
         return hipErrorInvalidValue;
-    const int64_t vecs = (int64_t)batch->max_rows * a.g;
     if (vecs > 32) {
-        a.nb = (int)pr_blocks(batch, a.kvh, a.rt);
+        a.nb = (int)pr_blocks(batch, a.kvh, a.g, w);
         a.work = work + 4 * (int64_t)a.nb;
-        return pool->bits == 16 ? pr_launch<16>(a, st)
-               : pool->bits == 8 ? pr_launch<8>(a, st) : pr_launch<4>(a, st);
+        if (w == 4) return pool->bits == 8 ? pr_launch<8, 4>(a, st) : pr_launch<4, 4>(a, st);
+        return pool->bits == 16 ? pr_launch<16, 8>(a, st)
+               : pool->bits == 8 ? pr_launch<8, 8>(a, st) : pr_launch<4, 8>(a, st);
     }
     a.work = work + ((batch->sessions + 3) & ~3);
     if (vecs <= 16 || pool->bits != 16)
