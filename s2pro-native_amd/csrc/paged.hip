@@ -16,6 +16,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "gemv_internal.h"
 #include "paged_dev.h"
 #include "prims_dev.h"
 
@@ -35,18 +36,28 @@ S2P_DEV float pa_max4(float v) { /* over the quad */
     return fmaxf(v, dpp_f<0x4E>(v));
 }
 
-template <int BW>
+/* two floats as a bf16 pair, one conversion for both */
+S2P_DEV uint32_t pa_pk(float a, float b) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f2;
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 b2;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
+}
+
+/* a wave: IT items (of four heads) of a row */
+template <int BW, int IT>
 __global__ __launch_bounds__(256) void k_paged_append(PgAppend a) {
 #pragma clang fp contract(off)
     const int lane = threadIdx.x & 63, j = lane & 15;
-    const int heads = a.qh + 2 * a.kvh, items = (heads + 3) >> 2;
-    const int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = __builtin_amdgcn_readfirstlane((int)(it / items));
+    const int heads = a.qh + 2 * a.kvh, waves = (heads + 4 * IT - 1) / (4 * IT); /* of a row */
+    const uint32_t wv = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = __builtin_amdgcn_readfirstlane((int)(wv / (uint32_t)waves));
     if (row >= a.b.rows) return;
-    const int head = ((int)(it % items) << 2) + (lane >> 4);
-    const bool live = head < heads;
-    s2p_u32x4 xw = {0u, 0u, 0u, 0u};
-    if (live) xw = *(const s2p_u32x4*)(a.qkv + ((size_t)row * heads + head) * PG_HD + 8 * j);
+    const int head0 = (int)(wv % (uint32_t)waves) * 4 * IT + (lane >> 4);
+    s2p_u32x4 xin[IT];
+#pragma unroll
+    for (int it = 0; it < IT; it++)
+        if (head0 + 4 * it < heads)
+            xin[it] = *(const s2p_u32x4*)(a.qkv + ((size_t)row * heads + head0 + 4 * it) * PG_HD + 8 * j);
     /* the row's session: as many as end at or before it */
     int s = 0;
     for (int i = 0; i < a.b.sessions; i += 64)
@@ -57,79 +68,97 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppend a) {
     if (i < 0 || i >= ss.n) return;
     const int slot = ss.L + i;
     const int p = a.pos ? a.pos[row] : slot;
-    if (p < 0 || p >= a.n_pos || !live) return;
-    const bool is_q = head < a.qh, is_v = head >= a.qh + a.kvh;
-    float x[8];
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        x[2 * k] = bf2f_lo(xw[k]);
-        x[2 * k + 1] = bf2f_hi(xw[k]);
-    }
-    if (!is_v) {
-        const uint16_t* w = is_q ? a.qn : a.kn;
-        if (w) {
-            float t[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                t[k] = fmaf(x[k], x[k], 0.f);
-                t[k] += dpp_f<0x128>(t[k]); /* row_ror:8 */
-                t[k] += dpp_f<0x124>(t[k]);
-                t[k] += dpp_f<0x122>(t[k]);
-                t[k] += dpp_f<0x121>(t[k]);
-            }
-            const float sum = ((t[0] + t[4]) + (t[2] + t[6])) + ((t[1] + t[5]) + (t[3] + t[7]));
-            const float inv = rsqrt_rule(sum / 128.0f + a.eps);
-            const s2p_u32x4 ww = *(const s2p_u32x4*)(w + 8 * j);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float wk = (k & 1) ? bf2f_hi(ww[k >> 1]) : bf2f_lo(ww[k >> 1]);
-                x[k] = bf2f(f2bf(__fmul_rn(__fmul_rn(x[k], inv), wk)));
-            }
-        }
-        const s2p_u32x4 cs = *(const s2p_u32x4*)(a.rope + (size_t)p * 64 + 4 * j);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float c = bf2f_lo(cs[k]), sn = bf2f_hi(cs[k]);
-            const float x0 = x[2 * k], x1 = x[2 * k + 1];
-            const float y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn));
-            const float y1 = __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, sn));
-            xw[k] = (uint32_t)f2bf(y0) | ((uint32_t)f2bf(y1) << 16);
-        }
-    }
-    if (is_q) {
-        *(s2p_u32x4*)(a.q + ((size_t)row * a.qh + head) * PG_HD + 8 * j) = xw;
-        return;
-    }
+    if (p < 0 || p >= a.n_pos) return;
     const int id = a.b.table[(size_t)s * a.b.max_pages + (slot >> a.l.shift)];
-    if ((unsigned)id >= (unsigned)a.l.pages) return;
-    const size_t at = (((size_t)id * a.l.planes + (head - a.qh)) << a.l.shift) +
-                      (slot & (a.l.page - 1));
-    if constexpr (BW == 16) {
-        *(s2p_u32x4*)(a.l.kv + at * 256 + 16 * j) = xw;
-    } else {
-        constexpr int QMAX = BW == 8 ? 127 : 7;
-        float m = 0.f;
+    const s2p_u32x4 cs = *(const s2p_u32x4*)(a.rope + (size_t)p * 64 + 4 * j);
+#pragma unroll
+    for (int it = 0; it < IT; it++) {
+        const int head = head0 + 4 * it;
+        if (head >= heads) return; /* nor the ones behind it */
+        const bool is_q = head < a.qh, is_v = head >= a.qh + a.kvh;
+        s2p_u32x4 xw = xin[it];
+        float x[8];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             x[2 * k] = bf2f_lo(xw[k]);
             x[2 * k + 1] = bf2f_hi(xw[k]);
-            m = fmaxf(m, fmaxf(fabsf(x[2 * k]), fabsf(x[2 * k + 1])));
         }
-        m = pa_max4(m);
-        const uint16_t hs = f2h(__fdiv_rn(m, (float)QMAX));
-        const float sc = h2f(hs);
-        uint32_t w[2] = {0u, 0u};
+        if (!is_v) {
+            const uint16_t* w = is_q ? a.qn : a.kn;
+            if (w) {
+                float t[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            int c = sc > 0.f ? (int)rintf(__fdiv_rn(x[k], sc)) : 0;
-            c = max(-QMAX, min(QMAX, c));
-            if (BW == 8) w[k >> 2] |= (uint32_t)(c & 0xFF) << (8 * (k & 3));
-            else w[0] |= (uint32_t)(c & 0xF) << (4 * k);
+                for (int k = 0; k < 8; k++) {
+                    t[k] = fmaf(x[k], x[k], 0.f);
+                    t[k] += dpp_f<0x128>(t[k]); /* row_ror:8 */
+                    t[k] += dpp_f<0x124>(t[k]);
+                    t[k] += dpp_f<0x122>(t[k]);
+                    t[k] += dpp_f<0x121>(t[k]);
+                }
+                const float sum = ((t[0] + t[4]) + (t[2] + t[6])) + ((t[1] + t[5]) + (t[3] + t[7]));
+                const float inv = rsqrt_rule(sum / 128.0f + a.eps);
+                const s2p_u32x4 ww = *(const s2p_u32x4*)(w + 8 * j);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t y = pa_pk(__fmul_rn(__fmul_rn(x[2 * k], inv), bf2f_lo(ww[k])),
+                                             __fmul_rn(__fmul_rn(x[2 * k + 1], inv), bf2f_hi(ww[k])));
+                    x[2 * k] = bf2f_lo(y);
+                    x[2 * k + 1] = bf2f_hi(y);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float c = bf2f_lo(cs[k]), sn = bf2f_hi(cs[k]);
+                const float x0 = x[2 * k], x1 = x[2 * k + 1];
+                xw[k] = pa_pk(__fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn)),
+                              __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, sn)));
+            }
         }
-        if constexpr (BW == 8) *(s2p_u32x2*)(a.l.kv + at * 128 + 8 * j) = (s2p_u32x2){w[0], w[1]};
-        else *(uint32_t*)(a.l.kv + at * 64 + 4 * j) = w[0];
-        if ((j & 3) == 0) a.l.sc[at * 4 + (j >> 2)] = hs;
+        if (is_q) {
+            *(s2p_u32x4*)(a.q + ((size_t)row * a.qh + head) * PG_HD + 8 * j) = xw;
+            continue;
+        }
+        if ((unsigned)id >= (unsigned)a.l.pages) continue;
+        const size_t at = (((size_t)id * a.l.planes + (head - a.qh)) << a.l.shift) +
+                          (slot & (a.l.page - 1));
+        if constexpr (BW == 16) {
+            *(s2p_u32x4*)(a.l.kv + at * 256 + 16 * j) = xw;
+        } else {
+            constexpr int QMAX = BW == 8 ? 127 : 7;
+            float m = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                x[2 * k] = bf2f_lo(xw[k]);
+                x[2 * k + 1] = bf2f_hi(xw[k]);
+                m = fmaxf(m, fmaxf(fabsf(x[2 * k]), fabsf(x[2 * k + 1])));
+            }
+            m = pa_max4(m);
+            const uint16_t hs = f2h(__fdiv_rn(m, (float)QMAX));
+            const float sc = h2f(hs);
+            uint32_t w[2] = {0u, 0u};
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                int c = sc > 0.f ? (int)rintf(__fdiv_rn(x[k], sc)) : 0;
+                c = max(-QMAX, min(QMAX, c));
+                if (BW == 8) w[k >> 2] |= (uint32_t)(c & 0xFF) << (8 * (k & 3));
+                else w[0] |= (uint32_t)(c & 0xF) << (4 * k);
+            }
+            if constexpr (BW == 8) *(s2p_u32x2*)(a.l.kv + at * 128 + 8 * j) = (s2p_u32x2){w[0], w[1]};
+            else *(uint32_t*)(a.l.kv + at * 64 + 4 * j) = w[0];
+            if ((j & 3) == 0) a.l.sc[at * 4 + (j >> 2)] = hs;
+        }
     }
+}
+
+template <int IT>
+static hipError_t pa_launch(const PgAppend& a, int bits, hipStream_t st) {
+    const int64_t waves = (int64_t)a.b.rows * ((a.qh + 2 * a.kvh + 4 * IT - 1) / (4 * IT));
+    if (waves > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)((waves + 3) / 4));
+    if (bits == 16) hipLaunchKernelGGL((k_paged_append<16, IT>), grid, dim3(256), 0, st, a);
+    else if (bits == 8) hipLaunchKernelGGL((k_paged_append<8, IT>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_append<4, IT>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 extern "C" hipError_t s2pk_paged_append(const s2p_page_pool* pool, const s2p_page_batch* batch,
@@ -156,13 +185,9 @@ extern "C" hipError_t s2pk_paged_append(const s2p_page_pool* pool, const s2p_pag
     a.n_pos = n_pos;
     a.qh = q_heads;
     a.kvh = pool->kv_heads;
-    const int64_t waves = (int64_t)batch->rows * ((q_heads + 2 * pool->kv_heads + 3) / 4);
-    if (waves > ((int64_t)1 << 31)) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)((waves + 3) / 4));
-    if (pool->bits == 16) hipLaunchKernelGGL(k_paged_append<16>, grid, dim3(256), 0, st, a);
-    else if (pool->bits == 8) hipLaunchKernelGGL(k_paged_append<8>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_paged_append<4>, grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    /* three items a wave share the row's lookups; one each where the chip is not full anyway */
+    return (int64_t)batch->rows * (q_heads + 2 * pool->kv_heads) > 128 * (int64_t)s2p_cu_count()
+               ? pa_launch<3>(a, pool->bits, st) : pa_launch<1>(a, pool->bits, st);
 }
 
 /* ------------------------------------------------------------ RoPE table */
