@@ -58,6 +58,11 @@ S2P_DEV uint32_t pd_pk(float a, float b) {
     typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 b2;
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
 }
+/* deq_int4 in one operation less: the sign bit's flip is in the constant that sets the exponent */
+S2P_DEV s2p_u32x4 pd_deq4(uint32_t d, uint32_t mask, uint32_t k) {
+    return (s2p_u32x4){((d << 3) & mask) ^ k, ((d >> 1) & mask) ^ k, ((d >> 5) & mask) ^ k,
+                       ((d >> 9) & mask) ^ k};
+}
 /* LDS reads of what global_load_lds wrote.  In C++ each would wait for every load in flight, the
  * next tile's too (the compiler does not tell the buffers apart), so they are written out, each
  * block with its own wait; what they read has arrived by pd_wait. */
@@ -426,7 +431,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
             int lane = threadIdx.x & 63;
             asm volatile("" : "+v"(lane));
             const int c = lane & 15, qq = lane >> 4;
-            uint32_t mask = 0x00780078u, one = 0x3F803F80u;
+            uint32_t mask = 0x00780078u, one = 0x3FC03FC0u;
             asm volatile("" : "+v"(mask), "+v"(one));
             const uint32_t v0 = pd_lds(vb), s0 = v0 + TS * EL + 8 * TS + 32 * qq;
             /* the row that the lane's address of a transposing read stands for */
@@ -480,8 +485,8 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
                         const s2p_u32x2 u = deq_s8(b[d].x), z = deq_s8(b[d].y);
                         va[0] = (s2p_u32x4){u.x, u.y, z.x, z.y};
                     } else {
-                        va[0] = deq_int4(b[d].x, mask, one);
-                        va[NH - 1] = deq_int4(b[d].y, mask, one);
+                        va[0] = pd_deq4(b[d].x, mask, one);
+                        va[NH - 1] = pd_deq4(b[d].y, mask, one);
                     }
 #pragma unroll
                     for (int qt = 0; qt < MQT; qt++)
@@ -538,7 +543,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
                         kd[2][0] = d2;
                         kd[3][0] = d3;
                     }
-                    uint32_t mask = 0x00780078u, one = 0x3F803F80u;
+                    uint32_t mask = 0x00780078u, one = 0x3FC03FC0u;
                     asm volatile("" : "+v"(mask), "+v"(one));
                     /* K scales of slots 16 p + 4 qq + 0 .. 3, four groups each */
                     s2p_u32x4 ks[2];
@@ -558,7 +563,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
                             const s2p_u32x2 u = deq_s8(kd[g][0]), w = deq_s8(kd[g][1]);
                             ka = (s2p_u32x4){u.x, u.y, w.x, w.y};
                         } else {
-                            ka = deq_int4(kd[g][0], mask, one);
+                            ka = pd_deq4(kd[g][0], mask, one);
                         }
 #pragma unroll
                         for (int qt = 0; qt < MQT; qt++) {
@@ -590,11 +595,6 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
 #pragma unroll
             for (int qt = 0; qt < MQT; qt++) {
                 float tm = -INFINITY;
-#pragma unroll
-                for (int p = 0; p < NP; p++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        x[qt][p][v] *= (BW == 4 ? 16.0f : 1.0f) * PD_SCALE;
                 uint64_t see = ~0ull;
                 if (!open) {
                     see = pd_mask(word[qt], ss.L - tb) & pd_groups(bad);
@@ -612,7 +612,8 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
                 for (int p = 0; p < NP; p++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) tm = fmaxf(tm, x[qt][p][v]);
-                tm = xg_max(tm);
+                constexpr float SC = (BW == 4 ? 16.0f : 1.0f) * PD_SCALE;
+                tm = xg_max(tm) * SC;
                 const float mn = fmaxf(m[qt], tm);
                 const float ms = mn == -INFINITY ? 0.f : mn;
                 const float corr = __builtin_amdgcn_exp2f(m[qt] - ms);
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(Pg
                 for (int p = 0; p < NP; p++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
-                        const float e = __builtin_amdgcn_exp2f(x[qt][p][v] - ms);
+                        const float e = __builtin_amdgcn_exp2f(fmaf(x[qt][p][v], SC, -ms));
                         ls += e;
                         x[qt][p][v] = e;
                     }
