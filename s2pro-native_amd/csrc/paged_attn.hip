@@ -268,7 +268,7 @@ S2P_DEV unsigned pd_swz(unsigned t) {
 }
 
 template <int BW, int MQT>
-__global__ __launch_bounds__(64 * PD_WAVES, BW == 8 ? 3 : 2) void k_paged_dec(PgAttn a) {
+__global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_paged_dec(PgAttn a) {
 #pragma clang fp contract(off)
     typedef PdTile<BW> Tile;
     constexpr int TS = Tile::TS, NG = Tile::NG, NP = Tile::NP, EL = Tile::EL, VB = Tile::VB;
@@ -1337,7 +1337,7 @@ template <int BW, int MQT>
 static hipError_t pd_launch(PgAttn a, hipStream_t st) {
     const int rnd = PdTile<BW>::TS * PD_WAVES;
     a.nvt = (a.b.max_rows * a.g + 16 * MQT - 1) / (16 * MQT);
-    a.nb = (int)pd_blocks(&a.b, a.kvh * a.nvt, rnd, BW == 8 ? 3 : 2);
+    a.nb = (int)pd_blocks(&a.b, a.kvh * a.nvt, rnd, BW == 8 && MQT == 1 ? 3 : 2);
     hipLaunchKernelGGL((k_paged_dec<BW, MQT>), dim3((unsigned)(a.nb * a.nvt * a.kvh)),
                        dim3(64 * PD_WAVES), 0, st, a);
     const hipError_t e = hipGetLastError();
@@ -1427,8 +1427,14 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
                : pool->bits == 8 ? pr_launch<8, 8>(a, st) : pr_launch<4, 8>(a, st);
     }
     a.work = work + ((batch->sessions + 3) & ~3);
-    if (vecs <= 16 || pool->bits != 16)
-        return pool->bits == 16 ? pd_launch<16, 1>(a, st)
-               : pool->bits == 8 ? pd_launch<8, 1>(a, st) : pd_launch<4, 1>(a, st);
-    return pd_launch<16, 2>(a, st);
+    /* 17 to 32 vectors: two tiles of them in a wave where its registers hold them.  INT4's do not
+     * (64-slot tiles; 16 sessions x 5 rows at 8,192 tokens take 145 us so, 72 with a block for each
+     * tile); INT8's spill a little, which pays from about six rounds a block on (the same 80 and
+     * 100 us; at 1,024 tokens 33 and 30). */
+    const bool two = vecs > 16 && (pool->bits == 16 || (pool->bits == 8 &&
+                     (int64_t)batch->sessions * ((batch->max_len + 127) / 128) * a.kvh >=
+                         6 * 2 * (int64_t)s2p_cu_count()));
+    if (two) return pool->bits == 16 ? pd_launch<16, 2>(a, st) : pd_launch<8, 2>(a, st);
+    return pool->bits == 16 ? pd_launch<16, 1>(a, st)
+           : pool->bits == 8 ? pd_launch<8, 1>(a, st) : pd_launch<4, 1>(a, st);
 }
