@@ -183,9 +183,9 @@ S2P_DEV int pd_batch(const PgAttn& a, int rnd, PdBatch& b) {
     return before;
 }
 
-/* A bf16 tile that not every row sees whole: V rows that are not there become zeros (what lies
- * behind a session may be NaN, and 0 x NaN is NaN), and a node's V row with a NaN or infinity
- * is added on its own to the vectors that see it, then zeroed for the matrix product. */
+/* A bf16 tile that not every row sees whole: V rows of pages that are not there become zeros, and
+ * a node's V row with a NaN or infinity is added on its own to the vectors that see it, then zeroed
+ * for the matrix product. */
 template <int MQT>
 S2P_DEV void pd_tail(const PgSess& ss, LDS(unsigned char)* vb, int tb, int bad,
                      const uint64_t (&seen)[MQT], const float (&x)[MQT][2][4],
@@ -197,9 +197,9 @@ S2P_DEV void pd_tail(const PgSess& ss, LDS(unsigned char)* vb, int tb, int bad,
         const int t = 4 * i + qq, j = tb + t;
         LDS(s2p_u32x4)* const p = (LDS(s2p_u32x4)*)(vb + i * 1024 + lane * 16);
         bool nf = false;
-        if (j >= ss.L + ss.n || ((bad >> (t >> 4)) & 1)) {
+        if ((bad >> (t >> 4)) & 1) {
             *p = (s2p_u32x4){0u, 0u, 0u, 0u};
-        } else if (j >= ss.L) {
+        } else if (j >= ss.L) { /* behind the nodes lies the last one again */
             const s2p_u32x4 w = *p;
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -362,16 +362,13 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
         const int n = nvec > 0 && tb0 < p1 ? (p1 - tb0 + RND - 1) / RND : 0;
         int ids = 0; /* lane x: the page of the wave's 16-slot group x (of 64 / NG tiles), or -1 */
         auto page_ids = [&](int k) __attribute__((always_inline)) {
-            const int slot = tb0 + (k + lane / NG) * RND + 16 * (lane % NG);
-            int id = -1;
-            if (slot < p1) {
-                id = tab[slot >> a.l.shift];
-                if ((unsigned)id >= (unsigned)a.l.pages) id = -1;
-            }
-            ids = id;
+            const int slot = min(tb0 + (k + lane / NG) * RND + 16 * (lane % NG), p1 - 1);
+            const int id = tab[slot >> a.l.shift];
+            ids = (unsigned)id < (unsigned)a.l.pages ? id : -1;
         };
-        /* tile k: K to registers, V (and scales) to buffer k & 1.  A group that is not there
-         * reads page 0 and is masked. */
+        /* tile k: K to registers, V (and scales) to buffer k & 1.  A page that is not there reads page
+         * 0 and is masked; behind the last slot the last one is read again (what lies there may be
+         * NaN, and 0 x NaN is NaN). */
         auto issue = [&](Tile& t, int k) __attribute__((always_inline)) {
             if ((k & (64 / NG - 1)) == 0) page_ids(k);
             unsigned lane = threadIdx.x & 63; /* offsets made here, not kept through the loop */
@@ -384,7 +381,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
             for (int g = 0; g < NG; g++) {
                 const int id = max(__builtin_amdgcn_readlane(ids, x0 + g), 0);
                 at[g] = (((uint64_t)(uint32_t)id * (uint32_t)a.l.planes + (uint32_t)kvh) << a.l.shift) +
-                        (uint32_t)((tb + 16 * g) & (a.l.page - 1));
+                        (uint32_t)(min(tb + 16 * g, (p1 - 1) & ~15) & (a.l.page - 1));
             }
             const uint64_t vplane = (uint64_t)(uint32_t)a.kvh << a.l.shift;
             if constexpr (BW != 16) {
@@ -411,8 +408,10 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
                 const unsigned t0 = i * (1024 / EL) % 16, tl = lane / (EL / 16);
                 const GblPtr vp = gbl_base(a.l.kv, (at[g] + vplane) * EL);
                 const unsigned ch = (lane % (EL / 16)) ^ pd_swz<BW>(i * (1024 / EL) + tl);
+                unsigned row = t0 + tl;
+                if constexpr (BW == 16) row = tb + 16 * g + 16 <= p1 ? row : min(row, (unsigned)(p1 - 1) & 15u);
                 __builtin_amdgcn_global_load_lds(
-                    (PgGlb*)(vp + (uint32_t)((t0 + tl) * EL + 16 * ch)),
+                    (PgGlb*)(vp + (uint32_t)(row * EL + 16 * ch)),
                     (PgLds*)(vb + i * 1024), 16, 0, 2 /* nontemporal */);
             }
         };
@@ -635,7 +634,7 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
             }
             if constexpr (BW == 16) {
                 s2p_u32x4 pw[MQT];
-                if (!open) pd_tail<MQT>(ss, (LDS(unsigned char)*)vb, tb, bad, seen, x, o);
+                if ((ss.n > 1 || a.vis || bad) && !open) pd_tail<MQT>(ss, (LDS(unsigned char)*)vb, tb, bad, seen, x, o);
 #pragma unroll
                 for (int qt = 0; qt < MQT; qt++)
 #pragma unroll
