@@ -38,7 +38,7 @@ typedef struct {
                        * 16-byte aligned */
     void*   scales;   /* bits 8 / 4: f16 [layers][pages][2 * kv_heads][page][4], 16-byte
                        * aligned; NULL with bits 16 */
-    int32_t layers, pages, kv_heads; /* pages <= 2^28, kv_heads <= 1024 */
+    int32_t layers, pages, kv_heads; /* pages <= 2^21, kv_heads <= 1024 */
     int32_t page;     /* slots a page: 16, 32, 64, 128 or 256 */
     int32_t bits;     /* 16, 8 or 4 */
 } s2p_page_pool;
@@ -58,7 +58,7 @@ typedef struct {
     int32_t max_pages;
     int32_t rows;          /* of the row arrays */
     int32_t max_rows;      /* host bound of a session's rows */
-    int32_t max_len;       /* host bound of len + rows, <= max_pages * page */
+    int32_t max_len;       /* host bound of len + rows, <= max_pages * page, <= 2^30 */
 } s2p_page_batch;
 
 /* bytes of the pool's kv and scales */
@@ -108,9 +108,10 @@ hipError_t s2pk_paged_commit(const s2p_page_pool* pool, const s2p_page_batch* ba
 
 /* The pages' bookkeeping, device resident.  ref counts the sessions that hold a page
  * (0: free); session s holds table[s][0 .. held[s] - 1], which cover its len[s]
- * tokens.  A program starts from zeros in ref, held and len.  Every session that
- * holds pages of the pool is a row here.  Calls on one set of tables are ordered by
- * their stream. */
+ * tokens.  A program starts from zeros in ref, held and len, raises len as it writes
+ * tokens into the room it reserved, and lowers it through s2pk_pages_free alone.  Every
+ * session that holds pages of the pool is a row here.  Calls on one set of tables are
+ * ordered by their stream. */
 typedef struct {
     int32_t* ref;    /* [pages] */
     int32_t* table;  /* [sessions][max_pages] */

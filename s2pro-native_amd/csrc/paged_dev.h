@@ -16,14 +16,14 @@ static inline bool pg_pool_ok(const s2p_page_pool* p) {
     if (p->bits != 16 && p->bits != 8 && p->bits != 4) return false;
     if (p->bits != 16 && (!p->scales || ((uintptr_t)p->scales & 15))) return false;
     if (p->page < 16 || p->page > 256 || (p->page & (p->page - 1))) return false;
-    /* pages: a scan's next round still counts in 32 bits; kv_heads: planes a page */
-    return p->layers > 0 && p->pages > 0 && p->pages <= 1 << 28 && p->kv_heads > 0 &&
+    /* pages: 1,024 sessions' needs of them are summed in 32 bits */
+    return p->layers > 0 && p->pages > 0 && p->pages <= 1 << 21 && p->kv_heads > 0 &&
            p->kv_heads <= 1024;
 }
 static inline bool pg_batch_ok(const s2p_page_pool* p, const s2p_page_batch* b) {
     if (!b || !b->table || !b->len || !b->row0) return false;
     if (b->sessions <= 0 || b->sessions > S2P_PAGE_MAX_SESSIONS || b->max_pages <= 0) return false;
-    if (b->max_rows <= 0 || b->max_rows > b->max_len) return false;
+    if (b->max_rows <= 0 || b->max_rows > b->max_len || b->max_len > 1 << 30) return false;
     return (int64_t)b->max_len <= (int64_t)b->max_pages * p->page;
 }
 /* query heads a kv head; 0: a grouping there is none of */

@@ -18,18 +18,28 @@
 #define PT_EACH 8   /* counts a thread takes at a time */
 #define PC_PIECE 16384
 
+/* inclusive sum over the 64 lanes, on the vector unit: within rows of 16, then the rows' last
+ * lanes to the rows behind */
+template <int CTRL, int ROWS>
+S2P_DEV uint32_t add_dpp(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+S2P_DEV uint32_t wave_scan(uint32_t v) {
+    v = add_dpp<0x111, 0xF>(v); /* row_shr:1 */
+    v = add_dpp<0x112, 0xF>(v);
+    v = add_dpp<0x114, 0xF>(v);
+    v = add_dpp<0x118, 0xF>(v);
+    v = add_dpp<0x142, 0xA>(v); /* row_bcast:15 into rows 1, 3 */
+    return add_dpp<0x143, 0xC>(v); /* row_bcast:31 into rows 2, 3 */
+}
 /* inclusive sum over the block; *total for everybody */
-S2P_DEV int64_t block_scan(int64_t v, int64_t* lds, int64_t* total) {
+S2P_DEV uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t t = __shfl_up(v, off, 64);
-        if (lane >= off) v += t;
-    }
+    v = wave_scan(v);
     __syncthreads(); /* lds may still be read from the scan before */
     if (lane == 63) lds[wave] = v;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    uint32_t before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < PT / 64; w++) {
         if (w < wave) before += lds[w];
@@ -52,16 +62,18 @@ S2P_DEV unsigned page_mask(const int32_t* ref, int i, int pages) {
 }
 
 /* work: [0] pairs, [4 ..) sources, then destinations (sessions each), then the free
- * pages in order */
+ * pages in order (those past the first PT_NEAR, which stay in LDS) */
+#define PT_NEAR 4096
 __global__ __launch_bounds__(PT) void k_pages_reserve(s2p_page_tables t, int pages, int shift,
                                                       const int32_t* __restrict__ want,
                                                       int32_t* __restrict__ granted,
                                                       int32_t* __restrict__ work) {
-    __shared__ int64_t s_scan[PT / 64];
-    __shared__ int64_t s_upto[PT]; /* pages needed by the sessions up to this one */
-    __shared__ int s_mine[PT];     /* the session's partly filled page, or -1 */
-    __shared__ int s_held[PT], s_copy[PT], s_rank[PT];
+    __shared__ __align__(16) uint32_t s_scan[PT / 64];
+    __shared__ uint32_t s_upto[PT]; /* pages needed by the sessions up to this one */
+    __shared__ __align__(16) int s_mine[PT]; /* the session's partly filled page, or -1 */
+    __shared__ int s_held[PT], s_len[PT], s_copy[PT], s_rank[PT], s_free[PT_NEAR];
     const int s = threadIdx.x, page = 1 << shift;
+    unsigned near = page_mask<true>(t.ref, s * PT_EACH, pages); /* on its way from the start */
     int held = 0, L = 0, more = 0, mine = -1, copy = 0;
     bool fits = false;
     if (s < t.sessions) {
@@ -85,27 +97,36 @@ __global__ __launch_bounds__(PT) void k_pages_reserve(s2p_page_tables t, int pag
             }
         }
     }
+    const int holders = mine >= 0 ? t.ref[mine] : 0;
     s_mine[s] = mine;
     s_held[s] = held;
+    s_len[s] = L;
     __syncthreads();
-    if (mine >= 0) { /* all but the last of a page's holders copy it */
+    if (holders > 1) { /* all but the last of a page's holders copy it */
         int before = 0;
-        for (int u = 0; u < s; u++) before += s_mine[u] == mine;
-        copy = before < t.ref[mine] - 1;
+        for (int u = 0; u < s; u += 4) {
+            const int4 m = *(const int4*)&s_mine[u];
+            before += (m.x == mine) + (u + 1 < s && m.y == mine) + (u + 2 < s && m.z == mine) +
+                      (u + 3 < s && m.w == mine);
+        }
+        copy = before < holders - 1;
     }
-    int64_t total, found = 0;
-    const int64_t need = more + copy;
+    /* 32 bits hold 1,024 sessions' needs, none counted for more than one page over all there are */
+    uint32_t total, found = 0;
+    const uint32_t need = min((uint32_t)more + (uint32_t)copy, (uint32_t)pages + 1);
     s_upto[s] = block_scan(need, s_scan, &total);
     /* the free pages, in order, until there are enough */
     int32_t* const fre = work + 4 + 2 * t.sessions;
     for (int i0 = 0; i0 < pages && found < total; i0 += PT * PT_EACH) {
         const int i = i0 + s * PT_EACH;
-        unsigned m = page_mask<true>(t.ref, i, pages);
+        unsigned m = i0 ? page_mask<true>(t.ref, i, pages) : near;
         const int c = __popc(m);
-        int64_t n;
-        int64_t at = found + block_scan(c, s_scan, &n) - c;
+        uint32_t n, at = found + block_scan(c, s_scan, &n) - c;
         while (m) {
-            fre[at++] = i + __ffs(m) - 1;
+            const int id = i + __ffs(m) - 1;
+            if (at < PT_NEAR) s_free[at] = id;
+            else fre[at] = id;
+            at++;
             m &= m - 1;
         }
         found += n;
@@ -114,31 +135,26 @@ __global__ __launch_bounds__(PT) void k_pages_reserve(s2p_page_tables t, int pag
     const bool ok = fits && s_upto[s] <= found;
     if (!ok) copy = 0;
     s_copy[s] = copy;
-    int64_t pairs;
-    const int pair = (int)block_scan(copy, s_scan, &pairs) - copy;
-    s_rank[s] = pair;
+    uint32_t pairs, give; /* what is granted is a prefix of the needs */
+    s_rank[s] = (int)block_scan(copy, s_scan, &pairs) - copy;
+    block_scan(ok ? need : 0, s_scan, &give);
     if (s == 0) work[0] = (int)pairs;
     if (granted && s < t.sessions) granted[s] = ok ? 1 : 0;
     if (ok) t.held[s] = held + more;
-    /* what is granted is a prefix of the needs */
-    int64_t give;
-    block_scan(ok ? need : 0, s_scan, &give);
     __syncthreads();
-    for (int64_t r = s; r < give; r += PT) {
+    for (uint32_t r = s; r < give; r += PT) {
         int lo = 0, hi = t.sessions - 1; /* the first session whose needs reach past r */
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (s_upto[mid] > r) hi = mid;
             else lo = mid + 1;
         }
-        const int k = (int)(r - (lo ? s_upto[lo - 1] : 0)), id = fre[r];
+        const int k = (int)(r - (lo ? s_upto[lo - 1] : 0)), id = r < PT_NEAR ? s_free[r] : fre[r];
         int32_t* row = t.table + (size_t)lo * t.max_pages;
         t.ref[id] = 1;
         if (k < s_copy[lo]) {
             const int old = s_mine[lo];
-            int at = 0; /* the place of the partly filled page: the one that covers len */
-            at = t.len[lo] >> shift;
-            row[at] = id;
+            row[s_len[lo] >> shift] = id;
             work[4 + s_rank[lo]] = old;
             work[4 + t.sessions + s_rank[lo]] = id;
             atomicSub(t.ref + old, 1);
@@ -267,14 +283,14 @@ __global__ __launch_bounds__(256) void k_pages_free(s2p_page_tables t, int pages
 __global__ __launch_bounds__(PT) void k_pages_plan(int32_t* __restrict__ ref, int pages,
                                                    int32_t* __restrict__ n_live,
                                                    int32_t* __restrict__ work) {
-    __shared__ int64_t s_scan[PT / 64];
+    __shared__ __align__(16) uint32_t s_scan[PT / 64];
     const int tid = threadIdx.x;
-    int64_t mine = 0, live;
+    uint32_t mine = 0, live;
     for (int64_t i = (int64_t)tid * PT_EACH; i < pages; i += PT * PT_EACH)
         mine += __popc(page_mask<false>(ref, (int)i, pages));
     block_scan(mine, s_scan, &live);
     int32_t *src = work + 4, *dst = src + pages / 2 + 1, *to = dst + pages / 2 + 1;
-    int64_t holes = 0, movers = 0;
+    uint32_t holes = 0, movers = 0;
     for (int64_t i0 = 0; i0 < pages; i0 += PT * PT_EACH) {
         const int64_t i = i0 + tid * PT_EACH;
         unsigned used = i < pages ? page_mask<false>(ref, (int)i, pages) : 0u;
@@ -282,11 +298,11 @@ __global__ __launch_bounds__(PT) void k_pages_plan(int32_t* __restrict__ ref, in
         for (int k = 0; k < PT_EACH; k++)
             if (i + k < live) front |= 1u << k;
         unsigned h = ~used & front, m = used & ~front;
-        /* both counts in one scan */
-        int64_t all;
-        const int64_t c = (int64_t)__popc(h) | ((int64_t)__popc(m) << 32);
-        const int64_t at = block_scan(c, s_scan, &all) - c;
-        int64_t ah = holes + (at & 0xFFFFFFFF), am = movers + (at >> 32);
+        /* both counts (8,192 at most) in one scan */
+        uint32_t all;
+        const uint32_t c = (uint32_t)__popc(h) | ((uint32_t)__popc(m) << 16);
+        const uint32_t at = block_scan(c, s_scan, &all) - c;
+        uint32_t ah = holes + (at & 0xFFFF), am = movers + (at >> 16);
         while (h) {
             dst[ah++] = (int)(i + __ffs(h) - 1);
             h &= h - 1;
@@ -295,11 +311,11 @@ __global__ __launch_bounds__(PT) void k_pages_plan(int32_t* __restrict__ ref, in
             src[am++] = (int)(i + __ffs(m) - 1);
             m &= m - 1;
         }
-        holes += all & 0xFFFFFFFF;
-        movers += all >> 32;
+        holes += all & 0xFFFF;
+        movers += all >> 16;
     }
     __syncthreads();
-    for (int64_t k = tid; k < movers; k += PT) { /* as many holes as movers */
+    for (uint32_t k = tid; k < movers; k += PT) { /* as many holes as movers */
         const int a = src[k], b = dst[k];
         to[a - live] = b;
         ref[b] = ref[a];

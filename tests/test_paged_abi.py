@@ -32,7 +32,7 @@ def tables(**kw):
 
 BAD_POOL = [dict(kv=None), dict(kv=A + 8), dict(bits=5), dict(bits=8), dict(bits=4, scales=A + 8),
             dict(page=8), dict(page=48), dict(page=512), dict(page=0), dict(layers=0),
-            dict(pages=0), dict(pages=-1), dict(pages=(1 << 28) + 1), dict(kv_heads=0),
+            dict(pages=0), dict(pages=-1), dict(pages=(1 << 21) + 1), dict(kv_heads=0),
             dict(kv_heads=2000)]
 BAD_BATCH = [dict(table=None), dict(len=None), dict(row0=None), dict(sessions=0),
              dict(sessions=1025), dict(max_pages=0), dict(max_rows=0), dict(max_len=0),
