@@ -857,7 +857,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
     constexpr int NC = BW == 16 ? 1 : BW == 8 ? 2 : 4;         /* 8-dim chunks of a piece */
     __shared__ __align__(256) uint16_t s_k[2][PR_TS * PG_HD], s_v[2][PR_TS * PG_HD];
     __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[W];
-    __shared__ unsigned long long s_odd[3]; /* bf16: nodes whose V holds a NaN or infinity */
+    /* bf16: nodes whose V holds a NaN or infinity; codes: a K scale over 512 */
+    __shared__ unsigned long long s_odd[3];
     __shared__ __align__(16) uint16_t s_vs[BW == 16 ? 1 : 2][PR_TS][4]; /* codes: V scales */
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -941,8 +942,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             for (int ks = 0; ks < 8; ks++)
                 qb[ks] = live ? *(const s2p_u32x4*)(qr + 16 * ks) : (s2p_u32x4){0u, 0u, 0u, 0u};
             if constexpr (BW != 16) {
-                /* q in f16: exact (11 bits for 8) below 2^15, larger vectors as multiples of a
-                 * power of two; the power, and K's 2^-7, go into the scale */
+                /* q in f16 as a multiple of a power of two (which goes into the scale): its largest
+                 * value at 2^14, all of its 8 bits down to 2^-28 of that */
                 uint32_t top = 0;
 #pragma unroll
                 for (int ks = 0; ks < 8; ks++)
@@ -950,9 +951,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                     for (int e = 0; e < 4; e++)
                         top = max(top, max(qb[ks][e] & 0x7FFFu, (qb[ks][e] >> 16) & 0x7FFFu));
                 top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-                const int up = min(max((int)(top >> 7) - (127 + 14), 0), 112);
+                const int up = min(max((int)(top >> 7) - (127 + 14), -112), 112);
                 const float down = __uint_as_float((uint32_t)(127 - up) << 23);
-                scale *= __uint_as_float((uint32_t)(127 + 7) << 23) * __uint_as_float((uint32_t)(127 + up) << 23);
+                scale *= __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
                 for (int ks = 0; ks < 8; ks++)
 #pragma unroll
@@ -1002,28 +1003,33 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         auto bad_of = [&](int k) __attribute__((always_inline)) {
             return (int)((__ballot(ids < 0) >> (((k - k0) & 15) * 4)) & 15);
         };
-        /* tile k to LDS.  Codes: K x scale x 2^-7 in f16 (never past its range, 2^-12 off), V's codes
-         * in bf16 (exact) and their scales.  bf16: V rows that are not there become zeros (what
-         * lies there may be NaN, and 0 x NaN is NaN), and so do pieces of a node's V with a NaN or
-         * infinity, which the rows that see the node add by themselves. */
-        auto store_k = [&](Stage& t, int buf) __attribute__((always_inline)) {
+        /* tile k to LDS.  Codes: K x scale in f16 (2^-12 off; a tile with a scale over 512 is marked
+         * and brought again as 2^-7 of itself, which stays in range), V's codes in bf16 (exact) and
+         * their scales.  bf16: V rows that are not there become zeros (what lies there may be NaN,
+         * and 0 x NaN is NaN), and so do pieces of a node's V with a NaN or infinity, which the rows
+         * that see the node add by themselves. */
+        auto put_k = [&](s2p_u32x4 w16, float ks, int trow, int ch, int buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < NC; e++) {
+                s2p_u32x4 w = w16;
+                if constexpr (BW != 16) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const uint32_t x = BW == 8 ? w16[2 * e + (q >> 1)] : w16[e];
+                        w[q] = pr_pk_f16(pr_code<BW>(x, q, 0) * ks, pr_code<BW>(x, q, 1) * ks);
+                    }
+                }
+                *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = w;
+            }
+        };
+        auto store_k = [&](Stage& t, int buf, int slot3) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
                 if (Stage::NP % (64 * W) && i >= Stage::NP) break;
-                const float ks = BW == 16 ? 1.f : h2f(t.s[j]) * 0.0078125f;
-#pragma unroll
-                for (int e = 0; e < NC; e++) {
-                    s2p_u32x4 w = t.w[j];
-                    if constexpr (BW != 16) {
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint32_t x = BW == 8 ? t.w[j][2 * e + (q >> 1)] : t.w[j][e];
-                            w[q] = pr_pk_f16(pr_code<BW>(x, q, 0) * ks, pr_code<BW>(x, q, 1) * ks);
-                        }
-                    }
-                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = w;
-                }
+                if constexpr (BW != 16)
+                    if (t.s[j] > 0x6000u && t.s[j] < 0x7C00u) s_odd[slot3] = 1; /* 512 < scale < inf */
+                put_k(t.w[j], BW == 16 ? 1.f : h2f(t.s[j]), trow, ch, buf);
             }
         };
         auto store_v = [&](Stage& t, int k, int buf, int bad, int slot3) __attribute__((always_inline)) {
@@ -1064,7 +1070,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         issue(sk, k0, false);
         issue(sv, k0, true);
         int bad = bad_of(k0), next = 0;
-        store_k(sk, 0);
+        store_k(sk, 0, seq);
         store_v(sv, k0, 0, bad, seq);
         if (k0 + 1 < k1) {
             issue(sk, k0 + 1, false);
@@ -1077,10 +1083,23 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             const LDS(uint16_t)* kt = (const LDS(uint16_t)*)s_k[buf];
             const LDS(uint16_t)* vt = (const LDS(uint16_t)*)s_v[buf];
             const int after = seq == 2 ? 0 : seq + 1;
-            unsigned long long odd = 0;
-            if constexpr (BW == 16) {
-                odd = s_odd[seq];
-                if (tid == 0) s_odd[seq ? seq - 1 : 2] = 0; /* everybody has read it, nobody set it again */
+            const unsigned long long odd = s_odd[seq];
+            if (tid == 0) s_odd[seq ? seq - 1 : 2] = 0; /* everybody has read it, nobody set it again */
+            float tscale = scale;
+            if constexpr (BW != 16) {
+                if (odd) { /* uniform and rare */
+                    for (int i = tid; i < Stage::NP; i += 64 * W) {
+                        const int trow = i / CR, ch = i % CR, slot = min(tb + trow, span - 1);
+                        int id = tab[slot >> a.l.shift];
+                        if ((unsigned)id >= (unsigned)a.l.pages) id = 0; /* masked */
+                        const size_t at = (((size_t)id * a.l.planes + kvh) << a.l.shift) +
+                                          (slot & (a.l.page - 1));
+                        const float ks = h2f(a.l.sc[at * 4 + (BW == 8 ? ch >> 1 : ch)]);
+                        put_k(*(const s2p_u32x4*)(a.l.kv + at * EL + 16 * ch), ks * 0.0078125f, trow, ch, buf);
+                    }
+                    tscale = scale * 128.0f;
+                    __syncthreads();
+                }
             }
             const bool work = busy && tb < wend;
             const bool open = tb + PR_TS <= open_end && bad == 0;
@@ -1149,7 +1168,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                 float tm = x[0];
 #pragma unroll
                 for (int i = 1; i < 16; i++) tm = fmaxf(tm, x[i]);
-                tm = pr_swap_max(tm) * scale;
+                tm = pr_swap_max(tm) * tscale;
                 if (__any(tm > m + PR_LAZY)) {
                     const float mn = tm > m + PR_LAZY ? tm : m;
                     const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -1162,7 +1181,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                 float ls = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale, -ms));
+                    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], tscale, -ms));
                     ls += x[i];
                 }
                 l += ls;
@@ -1241,7 +1260,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             }
             bad = next;
             if (k + 1 < k1) {
-                store_k(sk, buf ^ 1);
+                store_k(sk, buf ^ 1, after);
                 store_v(sv, k + 1, buf ^ 1, bad, after);
                 if (k + 2 < k1) {
                     page_ids(k + 2);

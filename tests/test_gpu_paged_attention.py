@@ -244,3 +244,54 @@ def test_a_long_session(lib):
     """33,000 slots; every split of it counts"""
     run(lib, 61, 4, 256, 1, 4, [33000, 10], [1, 1])
     run(lib, 62, 16, 128, 1, 4, [20000], [6])
+
+
+@pytest.mark.parametrize("bits,rows", [(16, 1), (8, 5), (4, 2), (16, 40), (8, 40), (4, 33)])
+def test_as_many_sessions_as_there_can_be(lib, bits, rows):
+    lens = [(31 * i) % 50 for i in range(1024)]
+    nrows = [rows if i % 97 == 5 else (i % 3 if rows > 1 else 1) for i in range(1024)]
+    run(lib, 71 + bits + rows, bits, 16, 1, 2, lens, nrows)
+
+
+@pytest.mark.parametrize("bits,rows", [(8, 1), (4, 1), (8, 40), (4, 40)])
+@pytest.mark.parametrize("kscale,qscale", [(2.0 ** 16, 2.0 ** -16), (2.0 ** 14, 2.0 ** -14), (2.0 ** 9, 2.0 ** -8),
+                                           (2.0 ** -4, 2.0 ** 6), (1.0, 2.0 ** 17)])
+def test_far_off_magnitudes_of_codes(lib, bits, rows, kscale, qscale):
+    """K scales of hundreds (values past 65,504), queries past f16's range: powers of two change
+    no rounding where the cache's scales stay normal"""
+    lens, nrows, page, kvh, g = [150, 20], [rows, 3], 32, 2, 4
+    pool = Pool(81 + bits, bits, pages_for(page, lens, nrows), kvh, page)
+    f = kscale if bits == 8 else kscale / 16
+    pool.scales[:, :, :kvh] = (pool.scales[:, :, :kvh].float() * f).to(torch.float16)
+    b = new_batch(8, pool.pages, page, lens, nrows)
+    q = rand_q(9, b.rows, kvh * g, qscale * (1 if qscale < 1e4 else 2.0 ** -17))
+    if qscale > 1e4:  # one vector of huge queries, orthogonal to all but a few dims
+        q = q.clone()
+        q.view(b.rows, kvh * g, 128)[0, 0, 3:] = 0
+        q.view(b.rows, kvh * g, 128)[0, 0, :3] = 2.0 ** 17
+        keep(q)
+    check(attend(lib, pool, b, q, kvh * g), *reference(pool, b, q, kvh * g))
+
+
+@pytest.mark.parametrize("bits,rows", [(16, 1), (8, 1), (4, 5), (16, 40), (8, 40), (4, 40)])
+def test_a_nan_query_stays_in_its_row_and_head(lib, bits, rows):
+    lens, nrows, page, kvh, g = [90, 30], [rows, rows], 16, 2, 4
+    pool = Pool(91 + bits, bits, pages_for(page, lens, nrows), kvh, page)
+    b = new_batch(10, pool.pages, page, lens, nrows)
+    q = rand_q(11, b.rows, kvh * g)
+    clean = attend(lib, pool, b, q, kvh * g).clone()
+    q.view(b.rows, kvh * g, 128)[rows - 1, 3, 17] = float("nan")
+    out = attend(lib, pool, b, q, kvh * g).view(b.rows, kvh * g, 128)
+    assert torch.isnan(out[rows - 1, 3].float()).all()
+    out[rows - 1, 3] = clean.view_as(out)[rows - 1, 3]
+    assert torch.equal(out.view_as(clean), clean)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_scores_that_are_all_minus_infinity(lib, rows):
+    """the softmax of nothing but -inf is NaN by its formula, unlike that of no slot"""
+    pool = Pool(95, 16, 4, 1, 16)
+    pool.kv[:, :, 0] = float("-inf")
+    b = Batch([[2, 1, 0]], [3], [rows], 16)
+    q = keep(torch.ones(rows, 2 * 128, dtype=torch.bfloat16, device=DEV))
+    assert torch.isnan(attend(lib, pool, b, q, 2).float()).all()
