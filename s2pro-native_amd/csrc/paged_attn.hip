@@ -5,7 +5,7 @@
  * over the slots j that the row sees, in one pass with the running maximum m.
  *
  * Up to 32 query vectors (rows x heads a kv head) a session, k_paged_dec: bound by the
- * K/V stream.  A block is a kv head's share of the rounds (four waves x a tile of 32
+ * K/V stream (over codes by their conversion).  A block is a kv head's share of the rounds (four waves x a tile of 32
  * bf16 or 64 coded slots) of all sessions, each block the same number of rounds, so
  * ragged lengths need no bound on the host and no session waits for the longest:
  *   - S^T = K Q^T on the matrix cores, K straight from HBM into the operand; the lane
@@ -16,7 +16,26 @@
  *   - INT8 codes convert exactly to bf16, INT4 codes to 1.5 + c / 16; a group's K scale
  *     multiplies its 32-dim partial score in f32, its V scale p before p's rounding;
  *   - p is rounded to bf16 (2^-9 of it, as the output is), the sums stay in f32.
- * A session that several blocks worked on is merged from their partials by k_paged_merge. */
+ * A session that several blocks worked on is merged from their partials by k_paged_merge.
+ *
+ * More query vectors, k_paged_rows: bound by the matrix cores and the softmax between
+ * their products.  A row tile is 256 vectors (128 over codes when no session has more);
+ * a wave takes 32 of them through every 64-slot tile of K and V, which the block shares
+ * in LDS:
+ *   - S^T = K Q^T and O^T = V^T P^T with 32 x 32 x 16 products, P in registers as above;
+ *   - one tile is worked on, one lies converted in LDS, one is on its way in registers,
+ *     so there is one barrier a tile;
+ *   - O follows a new maximum only when p would pass 2^8 (f32 has the room; p's and the
+ *     sums' relative precision do not depend on the maximum);
+ *   - codes become K x scale in f16 (11 bits), and q, which a wave scales by a power of
+ *     two, f16 without loss; V stays its exact code, its scale goes into p;
+ *   - the tiles of slots that all row tiles need are dealt out evenly over one round of
+ *     blocks, a row tile that several worked on is merged by k_paged_rows_merge.
+ *
+ * MI355X, 32 heads on 8 kv heads, in a stream of calls: 16 sessions x 8,192 tokens, one row
+ * each, bf16 87 us (6.2 TB/s); 32 over INT4 codes at 512 .. 4,096 tokens 32 us; one at 100
+ * tokens 5.8 us in a graph; 2 x 2,048 rows, half of them behind 2,048 tokens, 220 us
+ * (770 TFLOP/s; 190 with the softmax taken out); 4 x 17 rows at 8,192 tokens 44 us. */
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -58,7 +77,8 @@ S2P_DEV uint32_t pd_pk(float a, float b) {
     typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 b2;
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
 }
-/* deq_int4 in one operation less: the sign bit's flip is in the constant that sets the exponent */
+/* four INT4 codes a word to bf16 1.5 + c / 16: the code's bits into the mantissa, exponent and the
+ * sign bit's flip in one constant */
 S2P_DEV s2p_u32x4 pd_deq4(uint32_t d, uint32_t mask, uint32_t k) {
     return (s2p_u32x4){((d << 3) & mask) ^ k, ((d >> 1) & mask) ^ k, ((d >> 5) & mask) ^ k,
                        ((d >> 9) & mask) ^ k};
@@ -634,7 +654,8 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
             }
             if constexpr (BW == 16) {
                 s2p_u32x4 pw[MQT];
-                if ((ss.n > 1 || a.vis || bad) && !open) pd_tail<MQT>(ss, (LDS(unsigned char)*)vb, tb, bad, seen, x, o);
+                if ((ss.n > 1 || a.vis || bad) && !open)
+                    pd_tail<MQT>(ss, (LDS(unsigned char)*)vb, tb, bad, seen, x, o);
 #pragma unroll
                 for (int qt = 0; qt < MQT; qt++)
 #pragma unroll
@@ -791,6 +812,10 @@ __global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int tile) {
 /* ------------------------------------------------------------ many rows a session */
 
 #define PR_TS 64               /* slots of a tile */
+/* A row tile's start (q, the first loads with nothing to hide them) and end, in rounds of the
+ * schedule: without them 2,048 rows of one session from position 0 take 108 us, with three 82;
+ * 2 x 2,048 behind 2,048 tokens, whose tiles are long, 257 and 259. */
+#define PR_BEGIN 3
 #define PR_LAZY 8.0f           /* the running maximum follows when p would pass 2^8 */
 
 typedef __attribute__((ext_vector_type(16))) float pr_f32x16;
@@ -825,12 +850,11 @@ S2P_DEV bool pr_odd(s2p_u32x4 w) { /* eight bf16, one of them NaN or infinite */
         o |= (w[e] & 0x7F80u) == 0x7F80u || (w[e] & 0x7F800000u) == 0x7F800000u;
     return o;
 }
-/* tiles of slots that row tile r of a session needs */
+/* rounds that row tile r of a session costs: its tiles of slots, and PR_BEGIN before them */
 S2P_DEV int pr_rounds(const PgAttn& a, const PgSess& s, int r) {
     const int span = s.L + (a.vis ? s.n : min(s.n, (r + 1) * a.rt));
-    return (span + PR_TS - 1) / PR_TS;
+    return PR_BEGIN + (span + PR_TS - 1) / PR_TS;
 }
-
 /* a code pair's element of a word: INT8 word q / 2 of the chunk, INT4 the chunk's one word */
 template <int BW>
 S2P_DEV float pr_code(uint32_t w, int q, int e) {
@@ -920,6 +944,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             r++;
         }
         const int last = first + cnt, stop = min(end, last);
+        const int k0 = max(0, cur - first - PR_BEGIN), k1 = stop - first - PR_BEGIN;
+        cur = stop;
+        if (k1 <= 0) break; /* the block ends in the tile's first rounds: the next one begins it */
         const int i0 = r * a.rt, rows = min(a.rt, ss.n - i0); /* the tile's rows */
         const int span = ss.L + (a.vis ? ss.n : i0 + rows);   /* slots that one of them may see */
         const int32_t* tab = a.b.table + (size_t)s * a.b.max_pages;
@@ -969,8 +996,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
 #pragma unroll
             for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
 
-        const int k0 = cur - first, k1 = stop - first;
-        int ids = 0; /* lane x: the page of the 16-slot group x of 16 tiles, or -1 */
+        int ids = 0; /* of 16 tiles, 64 groups of 16 slots: lane x has group x's page, or -1 */
         auto page_ids = [&](int k) __attribute__((always_inline)) {
             if (((k - k0) & 15) == 0) {
                 const int slot = (k + (lane >> 2)) * PR_TS + 16 * (lane & 3);
@@ -1136,127 +1162,131 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                 const s2p_u32x2 b1 = ds_read_tr16((const LDS(uint16_t)*)(p + 2048));
                 return (s2p_u32x4){b0.x, b0.y, b1.x, b1.y};
             };
-            if (work) read_k(0);
+            if (work) {
+                read_k(0);
 #pragma unroll
-            for (int h = 0; h < 2; h++) { /* halves of 32 slots */
-              if (work) {
-                pr_f32x16 sc;
+                for (int h = 0; h < 2; h++) { /* halves of 32 slots */
+                    pr_f32x16 sc;
 #pragma unroll
-                for (int i = 0; i < 16; i++) sc[i] = 0.f;
+                    for (int i = 0; i < 16; i++) sc[i] = 0.f;
+                    /* the products go first: while a wave has them another one's softmax fills
+                     * the vector unit (2 x 2,048 rows 252 us, 259 without; around O's too: 261) */
+                    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int ks = 0; ks < 8; ks++)
-                    sc = BW == 16 ? mfma32x32x16(kr[ks], qb[ks], sc) : mfma32x32x16_f16(kr[ks], qb[ks], sc);
-                __builtin_amdgcn_sched_barrier(0);
-                /* the next operands are read while the softmax runs */
-                s2p_u32x4 vr[2][4];
-                if constexpr (BW == 16) {
-#pragma unroll
-                    for (int dt = 0; dt < 4; dt++) vr[0][dt] = read_v(2 * h, dt);
+                    for (int ks = 0; ks < 8; ks++)
+                        sc = BW == 16 ? mfma32x32x16(kr[ks], qb[ks], sc) : mfma32x32x16_f16(kr[ks], qb[ks], sc);
+                    __builtin_amdgcn_s_setprio(0);
                     __builtin_amdgcn_sched_barrier(0);
-                }
-                if (h == 0) read_k(1);
-                /* x[i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
-                float x[16];
+                    /* the next operands are read while the softmax runs */
+                    s2p_u32x4 vr[2][4];
+                    if constexpr (BW == 16) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = sc[i];
-                const uint32_t mine = (uint32_t)(seen >> (32 * h)) >> (4 * half);
-                if (!open) {
+                        for (int dt = 0; dt < 4; dt++) vr[0][dt] = read_v(2 * h, dt);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (h == 0) read_k(1);
+                    /* x[i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
+                    float x[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (!((mine >> (8 * (i >> 2) + (i & 3))) & 1)) x[i] = -INFINITY;
-                }
-                float tm = x[0];
+                    for (int i = 0; i < 16; i++) x[i] = sc[i];
+                    const uint32_t mine = (uint32_t)(seen >> (32 * h)) >> (4 * half);
+                    if (!open) {
 #pragma unroll
-                for (int i = 1; i < 16; i++) tm = fmaxf(tm, x[i]);
-                tm = pr_swap_max(tm) * tscale;
-                if (__any(tm > m + PR_LAZY)) {
-                    const float mn = tm > m + PR_LAZY ? tm : m;
-                    const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                    l *= corr;
+                        for (int i = 0; i < 16; i++)
+                            if (!((mine >> (8 * (i >> 2) + (i & 3))) & 1)) x[i] = -INFINITY;
+                    }
+                    float tm = x[0];
 #pragma unroll
-                    for (int dt = 0; dt < 4; dt++) o[dt] *= corr;
-                    m = mn;
-                }
-                const float ms = m == -INFINITY ? 0.f : m;
-                float ls = 0.f;
+                    for (int i = 1; i < 16; i++) tm = fmaxf(tm, x[i]);
+                    tm = pr_swap_max(tm) * tscale;
+                    if (__any(tm > m + PR_LAZY)) {
+                        const float mn = tm > m + PR_LAZY ? tm : m;
+                        const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                        l *= corr;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], tscale, -ms));
-                    ls += x[i];
-                }
-                l += ls;
-                if constexpr (BW == 16) {
-                    if (odd) { /* uniform and rare: what store() left out, from the page itself */
-                        for (uint32_t w = (uint32_t)(odd >> (32 * h)); w; w &= w - 1) {
-                            const int t = __ffs(w) - 1, slot = tb + 32 * h + t;
-                            float p = 0.f;
+                        for (int dt = 0; dt < 4; dt++) o[dt] *= corr;
+                        m = mn;
+                    }
+                    const float ms = m == -INFINITY ? 0.f : m;
+                    float ls = 0.f;
 #pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                p = (t >> 3) == (i >> 2) && (t & 3) == (i & 3) ? x[i] : p;
-                            p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
-                            if ((seen >> (32 * h + t)) & 1) {
-                                const int id = tab[slot >> a.l.shift]; /* there: its bit is set */
-                                const char* vp = a.l.kv +
-                                    ((((size_t)id * a.l.planes + a.kvh + kvh) << a.l.shift) +
-                                     (slot & (a.l.page - 1))) * EL;
+                    for (int i = 0; i < 16; i++) {
+                        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], tscale, -ms));
+                        ls += x[i];
+                    }
+                    l += ls;
+                    if constexpr (BW == 16) {
+                        if (odd) { /* uniform and rare: what store_v left out, from the page */
+                            for (uint32_t w = (uint32_t)(odd >> (32 * h)); w; w &= w - 1) {
+                                const int t = __ffs(w) - 1, slot = tb + 32 * h + t;
+                                float p = 0.f;
 #pragma unroll
-                                for (int i = 0; i < 16; i++) { /* o[i / 4], dims 8 (i % 4) + 4 half .. */
-                                    const s2p_u32x4 w8 = *(const s2p_u32x4*)(vp + 64 * (i >> 2) + 16 * (i & 3));
-                                    if (!pr_odd(w8)) continue;
+                                for (int i = 0; i < 16; i++)
+                                    p = (t >> 3) == (i >> 2) && (t & 3) == (i & 3) ? x[i] : p;
+                                p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
+                                if ((seen >> (32 * h + t)) & 1) {
+                                    const int id = tab[slot >> a.l.shift]; /* there: its bit is set */
+                                    const char* vp = a.l.kv +
+                                        ((((size_t)id * a.l.planes + a.kvh + kvh) << a.l.shift) +
+                                         (slot & (a.l.page - 1))) * EL;
 #pragma unroll
-                                    for (int e = 0; e < 4; e++) {
-                                        const uint32_t d = half ? w8[2 + (e >> 1)] : w8[e >> 1];
-                                        o[i >> 2][4 * (i & 3) + e] =
-                                            fmaf(p, e & 1 ? bf2f_hi(d) : bf2f_lo(d), o[i >> 2][4 * (i & 3) + e]);
+                                    for (int i = 0; i < 16; i++) { /* o[i / 4], dims 8 (i % 4) + 4 half .. */
+                                        const s2p_u32x4 w8 = *(const s2p_u32x4*)(vp + 64 * (i >> 2) + 16 * (i & 3));
+                                        if (!pr_odd(w8)) continue;
+#pragma unroll
+                                        for (int e = 0; e < 4; e++) {
+                                            const uint32_t d = half ? w8[2 + (e >> 1)] : w8[e >> 1];
+                                            o[i >> 2][4 * (i & 3) + e] =
+                                                fmaf(p, e & 1 ? bf2f_hi(d) : bf2f_lo(d), o[i >> 2][4 * (i & 3) + e]);
+                                        }
                                     }
                                 }
                             }
                         }
-                    }
 #pragma unroll
-                    for (int dt = 0; dt < 4; dt++) vr[1][dt] = read_v(2 * h + 1, dt);
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int dt = 0; dt < 4; dt++) vr[1][dt] = read_v(2 * h + 1, dt);
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const s2p_u32x4 pw = {pd_pk(x[8 * b], x[8 * b + 1]), pd_pk(x[8 * b + 2], x[8 * b + 3]),
-                                              pd_pk(x[8 * b + 4], x[8 * b + 5]), pd_pk(x[8 * b + 6], x[8 * b + 7])};
+                        for (int b = 0; b < 2; b++) {
+                            const s2p_u32x4 pw = {pd_pk(x[8 * b], x[8 * b + 1]), pd_pk(x[8 * b + 2], x[8 * b + 3]),
+                                                  pd_pk(x[8 * b + 4], x[8 * b + 5]), pd_pk(x[8 * b + 6], x[8 * b + 7])};
 #pragma unroll
-                        for (int dt = 0; dt < 4; dt++) o[dt] = mfma32x32x16(vr[b][dt], pw, o[dt]);
-                    }
-                } else {
-                    /* a scale group is a tile of 32 dims: p times the group's scale is its weight */
+                            for (int dt = 0; dt < 4; dt++) o[dt] = mfma32x32x16(vr[b][dt], pw, o[dt]);
+                        }
+                    } else {
+                        /* a scale group is a tile of 32 dims: p times the group's scale is its weight */
 #pragma unroll
-                    for (int gp = 0; gp < 2; gp++) {
-                        uint32_t vs[16]; /* scales of groups 2 gp, 2 gp + 1 of x[i]'s slot */
+                        for (int gp = 0; gp < 2; gp++) {
+                            uint32_t vs[16]; /* scales of groups 2 gp, 2 gp + 1 of x[i]'s slot */
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            vs[i] = *(const LDS(uint32_t)*)((const LDS(uint16_t)*)&s_vs[buf][0][0] +
-                                                            4 * (32 * h + 8 * (i >> 2) + 4 * half + (i & 3)) + 2 * gp);
+                            for (int i = 0; i < 16; i++)
+                                vs[i] = *(const LDS(uint32_t)*)((const LDS(uint16_t)*)&s_vs[buf][0][0] +
+                                                                4 * (32 * h + 8 * (i >> 2) + 4 * half + (i & 3)) + 2 * gp);
 #pragma unroll
-                        for (int g = 0; g < 2; g++) {
-                            const int dt = 2 * gp + g;
-                            s2p_u32x4 va[2];
+                            for (int g = 0; g < 2; g++) {
+                                const int dt = 2 * gp + g;
+                                s2p_u32x4 va[2];
 #pragma unroll
-                            for (int b = 0; b < 2; b++) va[b] = read_v(2 * h + b, dt);
-                            __builtin_amdgcn_sched_barrier(0);
+                                for (int b = 0; b < 2; b++) va[b] = read_v(2 * h + b, dt);
+                                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int b = 0; b < 2; b++) {
-                                s2p_u32x4 pw;
+                                for (int b = 0; b < 2; b++) {
+                                    s2p_u32x4 pw;
 #pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const int i = 8 * b + 2 * e;
-                                    pw[e] = pd_pk(fmaf(pd_half(vs[i], g), x[i], 0.f),
-                                                  fmaf(pd_half(vs[i + 1], g), x[i + 1], 0.f));
-                                    if (!open) /* a scale may be NaN where the slot is not seen */
-                                        pw[e] &= ((mine >> (8 * (i >> 2) + (i & 3))) & 1 ? 0xFFFFu : 0u) |
-                                                 ((mine >> (8 * (i >> 2) + (i & 3) + 1)) & 1 ? 0xFFFF0000u : 0u);
+                                    for (int e = 0; e < 4; e++) {
+                                        const int i = 8 * b + 2 * e;
+                                        pw[e] = pd_pk(fmaf(pd_half(vs[i], g), x[i], 0.f),
+                                                      fmaf(pd_half(vs[i + 1], g), x[i + 1], 0.f));
+                                        if (!open) /* a scale may be NaN where the slot is not seen */
+                                            pw[e] &= ((mine >> (8 * (i >> 2) + (i & 3))) & 1 ? 0xFFFFu : 0u) |
+                                                     ((mine >> (8 * (i >> 2) + (i & 3) + 1)) & 1 ? 0xFFFF0000u : 0u);
+                                    }
+                                    o[dt] = mfma32x32x16(va[b], pw, o[dt]);
                                 }
-                                o[dt] = mfma32x32x16(va[b], pw, o[dt]);
                             }
                         }
                     }
                 }
-              }
             }
             bad = next;
             if (k + 1 < k1) {
@@ -1275,7 +1305,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         /* out, or the partial of a tile that other blocks work on too */
         const float lt0 = pr_swap_sum(l);
         const float lt = m == -INFINITY ? (any ? 1.f : 0.f) : lt0; /* -inf everywhere, not nothing */
-        if (cur == first && stop == last) {
+        if (k0 == 0 && stop == last) {
             const float inv = m == -INFINITY ? (any ? NAN : 0.f) : 1.f / lt;
             if (live) {
                 uint16_t* out = a.out + ((size_t)row * a.qh + vhead) * PG_HD + 4 * half;
@@ -1288,7 +1318,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                                         pd_pk(o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv)};
             }
         } else {
-            float* const po = a.work + ((size_t)(kvh * a.nb + blk) * 2 + (cur == first ? 1 : 0)) *
+            float* const po = a.work + ((size_t)(kvh * a.nb + blk) * 2 + (k0 == 0 ? 1 : 0)) *
                                            ((size_t)VEC * (PG_HD + 2));
             if (live) {
                 if (half == 0) {
@@ -1303,13 +1333,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                         *(s2p_f32x4*)(pz + 32 * dt + 8 * q) =
                             (s2p_f32x4){o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
             }
-            if (cur == first && kvh == 0 && tid == 0) { /* what begins here and ends elsewhere */
+            if (k0 == 0 && kvh == 0 && tid == 0) { /* what begins here and ends elsewhere */
                 a.sums[4 * blk] = ss.r0 + i0;
                 a.sums[4 * blk + 2] = (int)(((int64_t)last * nb - 1) / total); /* its last block */
             }
-            if (cur == first) nvec_out = nvec;
+            if (k0 == 0) nvec_out = nvec;
         }
-        cur = stop;
     }
     if (kvh == 0 && tid == 0) a.sums[4 * blk + 1] = nvec_out;
 }
@@ -1384,7 +1413,7 @@ static int pr_waves(int64_t vecs, bool codes) { return codes && vecs <= 128 ? 4 
 static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int g, int w) {
     const int rt = 32 * w / g;
     const int64_t most = (int64_t)b->sessions * ((b->max_rows + rt - 1) / rt) *
-                         ((b->max_len + PR_TS - 1) / PR_TS);
+                         (PR_BEGIN + (b->max_len + PR_TS - 1) / PR_TS);
     int64_t nb = 8 / w * s2p_cu_count() / kv_heads;
     if (nb < 1) nb = 1;
     return nb < most ? nb : most;
@@ -1434,8 +1463,8 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
     const int w = pr_waves(vecs, pool->bits != 16);
     a.rt = 32 * w / a.g;
     /* rounds are counted in 32 bits */
-    if ((int64_t)batch->sessions * ((batch->max_rows + a.rt - 1) / a.rt) * ((batch->max_len + 63) / 64) >
-        1 << 30)
+    if ((int64_t)batch->sessions * ((batch->max_rows + a.rt - 1) / a.rt) *
+            (PR_BEGIN + (batch->max_len + PR_TS - 1) / PR_TS) > 1 << 30)
         return hipErrorInvalidValue;
     if (vecs > 32) {
         a.nb = (int)pr_blocks(batch, a.kvh, a.g, w);
