@@ -179,12 +179,12 @@ def test_sessions_left_out_and_padding(lib, most):
 
 @pytest.mark.parametrize("rows", [1, 33])
 def test_offsets_past_32_bits(lib, rows):
-    """the second layer of a pool of 6 GiB, pages behind 4 GiB"""
-    page, kvh, pages = 256, 8, 3072 + 5
+    """the second layer of a pool of 10 GiB, pages behind 4 GiB"""
+    page, kvh, pages = 256, 8, 2601
     kv = keep(torch.empty(2, pages, 2 * kvh, page, 128, dtype=torch.bfloat16, device=DEV))
     pool = Pool(1, 16, 2, kvh, page)
     pool.kv, pool.pages, pool.layers, pool.layer = kv, pages, 2, 1
-    ids = [pages - 1, 2900, 0]
+    ids = [pages - 1, 2500, 0]
     for i in ids:
         kv[1, i].normal_()
     b = Batch([ids], [2 * page + 100], [rows], page)
