@@ -89,8 +89,10 @@ hipError_t s2pk_paged_append(const s2p_page_pool* pool, const s2p_page_batch* ba
  * [0, len) and, with vis NULL, slots len .. len + i; else slot len + b where bit b of
  * vis[row] is set (max_rows <= 64; s2p_verify's visibility words).  The rows' own K/V
  * are in their slots already.  A row that sees no slot gets zeros.  NaN and infinities
- * in slots that a row does not see do not reach it.  work:
- * s2pk_paged_attention_work_floats floats, 16-byte aligned. */
+ * in slots that a row does not see do not reach it, and a session's bits do not depend on
+ * what lies behind its last slot.  work: s2pk_paged_attention_work_floats floats, 16-byte
+ * aligned.  Refused too: sessions x row tiles (max_rows in eights at worst) x 64-slot tiles
+ * of max_len past 2^30. */
 hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_page_batch* batch, int layer,
                                 const s2p_bf16* q, int q_heads, const uint64_t* vis,
                                 s2p_bf16* out, float* work, hipStream_t st);

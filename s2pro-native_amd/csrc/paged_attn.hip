@@ -1048,13 +1048,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                 *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = w;
             }
         };
-        auto store_k = [&](Stage& t, int buf, int slot3) __attribute__((always_inline)) {
+        auto store_k = [&](Stage& t, int k, int buf, int bad, int slot3) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
                 if (Stage::NP % (64 * W) && i >= Stage::NP) break;
-                if constexpr (BW != 16)
-                    if (t.s[j] > 0x6000u && t.s[j] < 0x7C00u) s_odd[slot3] = 1; /* 512 < scale < inf */
+                if constexpr (BW != 16) /* 512 < scale < inf, in a slot that is there */
+                    if (t.s[j] > 0x6000u && t.s[j] < 0x7C00u && k * PR_TS + trow < span &&
+                        !((bad >> (trow >> 4)) & 1))
+                        s_odd[slot3] = 1;
                 put_k(t.w[j], BW == 16 ? 1.f : h2f(t.s[j]), trow, ch, buf);
             }
         };
@@ -1096,7 +1098,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         issue(sk, k0, false);
         issue(sv, k0, true);
         int bad = bad_of(k0), next = 0;
-        store_k(sk, 0, seq);
+        store_k(sk, k0, 0, bad, seq);
         store_v(sv, k0, 0, bad, seq);
         if (k0 + 1 < k1) {
             issue(sk, k0 + 1, false);
@@ -1290,7 +1292,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             }
             bad = next;
             if (k + 1 < k1) {
-                store_k(sk, buf ^ 1, after);
+                store_k(sk, k + 1, buf ^ 1, bad, after);
                 store_v(sv, k + 1, buf ^ 1, bad, after);
                 if (k + 2 < k1) {
                     page_ids(k + 2);

@@ -295,3 +295,23 @@ def test_scores_that_are_all_minus_infinity(lib, rows):
     b = Batch([[2, 1, 0]], [3], [rows], 16)
     q = keep(torch.ones(rows, 2 * 128, dtype=torch.bfloat16, device=DEV))
     assert torch.isnan(attend(lib, pool, b, q, 2).float()).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [1, 5, 40, 100])
+def test_bits_do_not_depend_on_what_lies_behind_the_end(lib, bits, rows):
+    page, kvh, g = 64, 2, 4
+    lens, n = [70, 300, 1], [rows, 1, rows]
+    pool = Pool(51, bits, pages_for(page, lens, n), kvh, page)
+    b = new_batch(52, pool.pages, page, lens, n)
+    q = rand_q(53, b.rows, kvh * g)
+    outs = []
+    for fill in (0.0, 60000.0, float("nan")):
+        for s in range(len(lens)):
+            end = lens[s] + n[s]
+            if end % page:
+                t = pool.kv if bits == 16 else pool.scales
+                t[0, int(b.table[s, end // page]), :, end % page:] = fill
+        outs.append(attend(lib, pool, b, q, kvh * g))
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
