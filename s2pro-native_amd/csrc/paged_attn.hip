@@ -19,9 +19,9 @@
  * A session that several blocks worked on is merged from their partials by k_paged_merge.
  *
  * More query vectors, k_paged_rows: bound by the matrix cores and the softmax between
- * their products.  A row tile is 256 vectors (128 over codes when no session has more);
- * a wave takes 32 of them through every 64-slot tile of K and V, which the block shares
- * in LDS:
+ * their products.  A row tile is 256 vectors; a wave takes 32 of them through every
+ * 64-slot tile of K and V, which the block shares in LDS (128, and two waves for 32
+ * vectors, each with half of a tile's slots, when no session has more):
  *   - S^T = K Q^T and O^T = V^T P^T with 32 x 32 x 16 products, P in registers as above;
  *   - one tile is worked on, one lies converted in LDS, one is on its way in registers,
  *     so there is one barrier a tile;
@@ -33,9 +33,9 @@
  *     blocks, a row tile that several worked on is merged by k_paged_rows_merge.
  *
  * MI355X, 32 heads on 8 kv heads, in a stream of calls: 16 sessions x 8,192 tokens, one row
- * each, bf16 87 us (6.2 TB/s); 32 over INT4 codes at 512 .. 4,096 tokens 32 us; one at 100
+ * each, bf16 87 us (6.2 TB/s); 32 over INT4 codes at 512 .. 4,096 tokens 30 us; one at 100
  * tokens 5.8 us in a graph; 2 x 2,048 rows, half of them behind 2,048 tokens, 220 us
- * (770 TFLOP/s; 190 with the softmax taken out); 4 x 17 rows at 8,192 tokens 44 us. */
+ * (770 TFLOP/s; 190 with the softmax taken out); 4 x 17 rows at 8,192 tokens 42 us. */
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -211,24 +211,29 @@ S2P_DEV void pd_tail(const PgSess& ss, LDS(unsigned char)* vb, int tb, int bad,
                      const uint64_t (&seen)[MQT], const float (&x)[MQT][2][4],
                      s2p_f32x4 (&o)[MQT][8]) {
     const int lane = threadIdx.x & 63, qq = lane >> 4, c = lane & 15;
-    uint32_t odd = 0;
+    uint32_t nf = 0, odd = 0; /* nf: of this lane's 16 bytes of rows 4 i + qq */
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const int t = 4 * i + qq, j = tb + t;
         LDS(s2p_u32x4)* const p = (LDS(s2p_u32x4)*)(vb + i * 1024 + lane * 16);
-        bool nf = false;
-        if ((bad >> (t >> 4)) & 1) {
+        if ((bad >> (i >> 2)) & 1) { /* uniform */
             *p = (s2p_u32x4){0u, 0u, 0u, 0u};
-        } else if (j >= ss.L) { /* behind the nodes lies the last one again */
+        } else if (tb + 4 * i + 3 >= ss.L) { /* behind the nodes lies the last one again */
             const s2p_u32x4 w = *p;
+            bool x = false;
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                nf |= (w[e] & 0x7F80u) == 0x7F80u || (w[e] & 0x7F800000u) == 0x7F800000u;
+                x |= (w[e] & 0x7F80u) == 0x7F80u || (w[e] & 0x7F800000u) == 0x7F800000u;
+            nf |= (uint32_t)(x && tb + 4 * i + qq >= ss.L) << i;
         }
-        const uint64_t b = __ballot(nf);
+    }
+    if (__any(nf)) { /* rare */
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            if ((b >> (16 * r)) & 0xFFFFu) odd |= 1u << (4 * i + r);
+        for (int i = 0; i < 8; i++) {
+            const uint64_t b = __ballot((nf >> i) & 1);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if ((b >> (16 * r)) & 0xFFFFu) odd |= 1u << (4 * i + r);
+        }
     }
     wave_lds_sync();
     while (odd) {
@@ -285,6 +290,15 @@ S2P_DEV unsigned pd_swz(unsigned t) {
     if constexpr (BW == 16) return (t & 7) << 1;
     else if constexpr (BW == 8) return ((t >> 1) & 3) | (((t >> 4) & 1) << 2);
     else return (t >> 4) & 3;
+}
+
+/* four dims of a session's query vector; a vector that saw no slot (no mark) gets zeros, one whose
+ * every score is -inf NaN */
+S2P_DEV void pd_out(const PgAttn& a, int r0, int kvh, int vec, int d, s2p_f32x4 z, float M, float lt,
+                    float mark) {
+    const float inv = M == -INFINITY ? (mark > 0.f ? NAN : 0.f) : 1.f / lt;
+    *(s2p_u32x2*)(a.out + ((size_t)(r0 + vec / a.g) * a.qh + kvh * a.g + vec % a.g) * PG_HD + d) =
+        (s2p_u32x2){pd_pk(z[0] * inv, z[1] * inv), pd_pk(z[2] * inv, z[3] * inv)};
 }
 
 template <int BW, int MQT>
@@ -712,29 +726,37 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
             }
         }
         __syncthreads();
-        /* merge the waves: vector by vector, a dim a thread */
+        /* merge the waves, four dims of a vector a thread */
         const bool whole = cur == first && stop == last;
         float* const po = a.work + (((size_t)(kvh * a.nb + blk) * 2 + (cur == first ? 1 : 0)) * a.nvt + vt) *
                                        (16 * MQT * (PG_HD + 2));
-        for (int i = tid; i < nvec * PG_HD; i += 64 * PD_WAVES) {
-            const int vec = i >> 7, d = i & 127;
-            float M = s_ml[0][vec][0];
-#pragma unroll
-            for (int w = 1; w < PD_WAVES; w++) M = fmaxf(M, s_ml[w][vec][0]);
-            const float Ms = M == -INFINITY ? 0.f : M;
-            float lt = 0.f, z = 0.f, mark = 0.f;
+        for (int i = tid; i < nvec * (PG_HD / 4); i += 64 * PD_WAVES) {
+            const int vec = i >> 5, d = 4 * (i & 31);
+            float pm[PD_WAVES], pl[PD_WAVES], M = -INFINITY;
+            s2p_f32x4 pz[PD_WAVES];
 #pragma unroll
             for (int w = 0; w < PD_WAVES; w++) {
-                const float e = __builtin_amdgcn_exp2f(s_ml[w][vec][0] - Ms);
-                lt = fmaf(s_ml[w][vec][1], e, lt);
-                mark = fmaxf(mark, s_ml[w][vec][1]);
-                z = fmaf(so[pd_oidx(w * 16 * MQT + vec, d)], e, z);
+                pm[w] = s_ml[w][vec][0];
+                pl[w] = s_ml[w][vec][1];
+                pz[w] = *(const LDS(s2p_f32x4)*)(so + pd_oidx(w * 16 * MQT + vec, d));
+            }
+#pragma unroll
+            for (int w = 0; w < PD_WAVES; w++) M = fmaxf(M, pm[w]);
+            const float Ms = M == -INFINITY ? 0.f : M;
+            float lt = 0.f, mark = 0.f;
+            s2p_f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < PD_WAVES; w++) {
+                const float e = __builtin_amdgcn_exp2f(pm[w] - Ms);
+                lt = fmaf(pl[w], e, lt);
+                mark = fmaxf(mark, pl[w]);
+#pragma unroll
+                for (int v = 0; v < 4; v++) z[v] = fmaf(pz[w][v], e, z[v]);
             }
             if (whole) {
-                a.out[((size_t)(ss.r0 + (v0 + vec) / a.g) * a.qh + kvh * a.g + (v0 + vec) % a.g) * PG_HD + d] =
-                    f2bf(M == -INFINITY && mark == 0.f ? 0.f : z / lt);
+                pd_out(a, ss.r0, kvh, v0 + vec, d, z, M, lt, mark);
             } else {
-                po[16 * MQT * 2 + i] = z;
+                *(s2p_f32x4*)(po + 16 * MQT * 2 + 4 * i) = z;
                 if (d == 0) {
                     po[2 * vec] = M;
                     po[2 * vec + 1] = M == -INFINITY ? mark : lt;
@@ -746,71 +768,86 @@ __global__ __launch_bounds__(64 * PD_WAVES, BW == 8 && MQT == 1 ? 3 : 2) void k_
     }
 }
 
-/* Sessions that several blocks worked on: their partials, in the order of the blocks.
- * A block a (vector, kv head, session): four quarters of the blocks, a dim a thread. */
-__global__ __launch_bounds__(512) void k_paged_merge(PgAttn a, int tile) {
-    __shared__ float s_m[4], s_l[4], s_k[4], s_z[4][PG_HD];
-    const int vec = blockIdx.x, kvh = blockIdx.y, s = blockIdx.z;
-    const int tid = threadIdx.x, d = tid & 127, part = tid >> 7;
+/* partials joined: running maximum, sum, mark (> 0: a slot was seen) and four dims of O */
+struct PgSum {
+    float M = -INFINITY, lt = 0.f, mark = 0.f;
+    s2p_f32x4 z = {0.f, 0.f, 0.f, 0.f};
+};
+S2P_DEV void pd_add(PgSum& o, float m, float l, s2p_f32x4 z, float mark) {
+    const float mn = fmaxf(o.M, m), ms = mn == -INFINITY ? 0.f : mn;
+    const float e0 = __builtin_amdgcn_exp2f(o.M - ms), e1 = __builtin_amdgcn_exp2f(m - ms);
+    o.mark = fmaxf(o.mark, mark);
+    o.lt = fmaf(o.lt, e0, l * e1);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o.z[e] = fmaf(o.z[e], e0, z[e] * e1);
+    o.M = mn;
+}
+/* Partial j of a run j0 .. j1 that blocks of a kv head left lies at (2 j + (j == j0)) strides from
+ * `base`: vec's (m, l) at 2 vec, its O at 2 tile + 128 vec.  PARTS threads of 32 apart share the run
+ * (part j - j0 mod PARTS), four dims each. */
+template <int PARTS>
+S2P_DEV PgSum pd_gather(const float* base, size_t stride, int tile, int j0, int j1, int vec, int part,
+                        int d) {
+    PgSum o;
+    for (int jj = j0 + part; jj <= j1; jj += 4 * PARTS) { /* four partials' loads at a time */
+        float pm[4], pl[4];
+        s2p_f32x4 pz[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int j = min(jj + u * PARTS, j1);
+            const float* p = base + ((size_t)j * 2 + (j == j0 ? 1 : 0)) * stride;
+            pm[u] = p[2 * vec];
+            pl[u] = p[2 * vec + 1];
+            pz[u] = *(const s2p_f32x4*)(p + 2 * tile + vec * PG_HD + d);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (jj + u * PARTS <= j1) pd_add(o, pm[u], pl[u], pz[u], pl[u]);
+    }
+    return o;
+}
+
+/* Sessions that several blocks worked on: their partials.  A block: 8 / PM_PARTS vectors of a kv
+ * head and session, PM_PARTS threads of 32 apart share a vector's partials. */
+#define PM_PARTS 4
+#define PM_VECS (8 / PM_PARTS)
+__global__ __launch_bounds__(256) void k_paged_merge(PgAttn a, int tile) {
+    __shared__ float s_m[PM_VECS][PM_PARTS][3];
+    __shared__ s2p_f32x4 s_z[PM_VECS][PM_PARTS][32];
+    const int kvh = blockIdx.y, s = blockIdx.z;
+    const int tid = threadIdx.x, x = tid & 31, part = (tid >> 5) % PM_PARTS, u = (tid >> 5) / PM_PARTS;
+    const int vec = blockIdx.x * PM_VECS + u;
     const int total = a.sums[a.b.sessions - 1], last = a.sums[s], first = s ? a.sums[s - 1] : 0;
     const PgSess ss = pg_session(a.b, s);
-    if (vec >= ss.n * a.g) return;
+    if ((int)blockIdx.x * PM_VECS >= ss.n * a.g) return;
     /* block of a round: the last j whose first round, j total / nb, is not behind it */
     const int nb = min(a.nb, total);
     const int j0 = (int)((((int64_t)first + 1) * nb - 1) / total);
     const int j1 = (int)(((int64_t)last * nb - 1) / total);
     if (j0 == j1) return; /* one block had all of it */
+    const bool live = vec < ss.n * a.g;
     const size_t stride = (size_t)tile * (PG_HD + 2); /* of a tile's partial */
-    const float* const base = a.work + ((size_t)kvh * a.nb * 2 * a.nvt + vec / tile) * stride;
-    const int tv = vec % tile;
-    const int each = (j1 - j0 + 4) >> 2;
-    const int from = j0 + part * each, to = min(from + each, j1 + 1);
-    float M = -INFINITY, lt = 0.f, z = 0.f, mark = 0.f;
-    for (int jj = from; jj < to; jj += 4) { /* four partials' loads at a time */
-        float pm[4], pl[4], pz[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int j = min(jj + u, to - 1);
-            const float* p = base + ((size_t)j * 2 + (j == j0 ? 1 : 0)) * a.nvt * stride;
-            pm[u] = p[2 * tv];
-            pl[u] = p[2 * tv + 1];
-            pz[u] = p[2 * tile + tv * PG_HD + d];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            if (jj + u >= to) break;
-            const float mn = fmaxf(M, pm[u]), ms = mn == -INFINITY ? 0.f : mn;
-            const float e0 = __builtin_amdgcn_exp2f(M - ms), e1 = __builtin_amdgcn_exp2f(pm[u] - ms);
-            mark = fmaxf(mark, pl[u]);
-            lt = fmaf(lt, e0, pl[u] * e1);
-            z = fmaf(z, e0, pz[u] * e1);
-            M = mn;
-        }
+    PgSum o;
+    if (live)
+        o = pd_gather<PM_PARTS>(a.work + ((size_t)kvh * a.nb * 2 * a.nvt + vec / tile) * stride,
+                                a.nvt * stride, tile, j0, j1, vec % tile, part, 4 * x);
+    if (x == 0) {
+        s_m[u][part][0] = o.M;
+        s_m[u][part][1] = o.lt;
+        s_m[u][part][2] = o.mark;
     }
-    if (d == 0) {
-        s_m[part] = M;
-        s_l[part] = lt;
-        s_k[part] = mark;
-    }
-    s_z[part][d] = z;
+    s_z[u][part][x] = o.z;
     __syncthreads();
-    if (part) return;
-    M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const float Ms = M == -INFINITY ? 0.f : M;
-    lt = z = mark = 0.f;
+    if (part || !live) return;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float e = __builtin_amdgcn_exp2f(s_m[i] - Ms);
-        lt = fmaf(s_l[i], e, lt);
-        z = fmaf(s_z[i][d], e, z);
-        mark = fmaxf(mark, s_k[i]);
-    }
-    a.out[((size_t)(ss.r0 + vec / a.g) * a.qh + kvh * a.g + vec % a.g) * PG_HD + d] =
-        f2bf(M == -INFINITY && mark == 0.f ? 0.f : z / lt);
+    for (int i = 1; i < PM_PARTS; i++)
+        pd_add(o, s_m[u][i][0], s_m[u][i][1], s_z[u][i][x], s_m[u][i][2]);
+    pd_out(a, ss.r0, kvh, vec, 4 * x, o.z, o.M, o.lt, o.mark);
 }
 
 /* ------------------------------------------------------------ many rows a session */
 
+#define PR_W 8                 /* waves of a block */
 #define PR_TS 64               /* slots of a tile */
 /* A row tile's start (q, the first loads with nothing to hide them) and end, in rounds of the
  * schedule: without them 2,048 rows of one session from position 0 take 108 us, with three 82;
@@ -863,24 +900,25 @@ S2P_DEV float pr_code(uint32_t w, int q, int e) {
 }
 
 /* what a thread brings of a tile's K or V: 16-byte pieces and their scales */
-template <int BW, int W>
+template <int BW>
 struct PrStage {
     static constexpr int EL = BW == 16 ? 256 : BW == 8 ? 128 : 64;
     static constexpr int NP = PR_TS * EL / 16;                       /* pieces of a tile's K or V */
-    static constexpr int NL = (NP + 64 * W - 1) / (64 * W);
+    static constexpr int NL = (NP + 64 * PR_W - 1) / (64 * PR_W);
     s2p_u32x4 w[NL];
     uint16_t s[NL];
 };
 
-template <int BW, int W>
-__global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
+template <int BW, int SP>
+__global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
 #pragma clang fp contract(off)
-    typedef PrStage<BW, W> Stage;
-    constexpr int VEC = 32 * W; /* query vectors of a row tile */
+    typedef PrStage<BW> Stage;
+    constexpr int VEC = 32 * PR_W / SP; /* query vectors of a row tile */
     constexpr int EL = Stage::EL, NL = Stage::NL, CR = EL / 16; /* pieces of a row */
     constexpr int NC = BW == 16 ? 1 : BW == 8 ? 2 : 4;         /* 8-dim chunks of a piece */
     __shared__ __align__(256) uint16_t s_k[2][PR_TS * PG_HD], s_v[2][PR_TS * PG_HD];
-    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[W];
+    __shared__ float s_ml[SP == 2 ? VEC : 1][2];
+    __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[PR_W];
     /* bf16: nodes whose V holds a NaN or infinity; codes: a K scale over 512 */
     __shared__ unsigned long long s_odd[3];
     __shared__ __align__(16) uint16_t s_vs[BW == 16 ? 1 : 2][PR_TS][4]; /* codes: V scales */
@@ -891,7 +929,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
 
     /* the block's share of the rounds of all row tiles */
     int total = 0;
-    for (int base = 0; base < a.b.sessions; base += 64 * W) {
+    for (int base = 0; base < a.b.sessions; base += 64 * PR_W) {
         int v = 0;
         if (base + tid < a.b.sessions) {
             const PgSess ss = pg_session(a.b, base + tid);
@@ -907,7 +945,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         __syncthreads();
         int all = total;
 #pragma unroll
-        for (int w = 0; w < W; w++) {
+        for (int w = 0; w < PR_W; w++) {
             if (w < wave) v += s_w[w];
             all += s_w[w];
         }
@@ -924,7 +962,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
     const int begin = (int)((int64_t)blk * total / nb);
     const int end = (int)((int64_t)(blk + 1) * total / nb);
 
-    const int vec = 32 * wave + col; /* this lane's query vector of a row tile */
+    /* SP = 2: two waves have the same vectors, each half of a tile's slots */
+    const int vw = wave / SP, part = wave % SP;
+    const int vec = 32 * vw + col; /* this lane's query vector of a row tile */
     const int vi = vec / a.g, vhead = kvh * a.g + vec % a.g;
     int nvec_out = 0; /* of the row tile that the block leaves to another one */
     int seq = 0;      /* tiles so far, mod 3 */
@@ -952,14 +992,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         const int32_t* tab = a.b.table + (size_t)s * a.b.max_pages;
         const int nvec = rows * a.g;
         const bool live = vec < nvec;
-        const bool busy = 32 * wave < nvec; /* the wave has a vector */
+        const bool busy = 32 * vw < nvec; /* the wave has a vector */
         const int row = ss.r0 + i0 + (live ? vi : 0);
         /* the row's nodes as a word, or (causal) how many slots it sees */
         const uint64_t word = a.vis && live ? a.vis[row] & pd_ones(ss.n) : 0ull;
         const int sees = live ? ss.L + i0 + vi + 1 : 0;
         /* no row of the wave sees a slot from here on; every one sees those before `open` */
-        const int wend = a.vis ? span : min(span, ss.L + i0 + (min(32 * wave + 31, nvec - 1) / a.g) + 1);
-        const int open_end = a.vis ? ss.L : ss.L + i0 + 32 * wave / a.g + 1;
+        const int wend = a.vis ? span : min(span, ss.L + i0 + (min(32 * vw + 31, nvec - 1) / a.g) + 1);
+        const int open_end = a.vis ? ss.L : ss.L + i0 + 32 * vw / a.g + 1;
 
         s2p_u32x4 qb[8];
         float scale = PD_SCALE;
@@ -1012,8 +1052,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         auto issue = [&](Stage& t, int k, bool is_v) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
-                if (Stage::NP % (64 * W) && i >= Stage::NP) break; /* whole waves */
+                const int i = tid + 64 * PR_W * j, trow = i / CR, ch = i % CR;
+                if (Stage::NP % (64 * PR_W) && i >= Stage::NP) break; /* whole waves */
                 const int g = __builtin_amdgcn_readfirstlane(trow >> 4); /* one group a wave */
                 const int id = max(__builtin_amdgcn_readlane(ids, ((k - k0) & 15) * 4 + g), 0);
                 const uint64_t at = (((uint64_t)(uint32_t)id * (uint32_t)a.l.planes +
@@ -1051,8 +1091,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         auto store_k = [&](Stage& t, int k, int buf, int bad, int slot3) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
-                if (Stage::NP % (64 * W) && i >= Stage::NP) break;
+                const int i = tid + 64 * PR_W * j, trow = i / CR, ch = i % CR;
+                if (Stage::NP % (64 * PR_W) && i >= Stage::NP) break;
                 if constexpr (BW != 16) /* 512 < scale < inf, in a slot that is there */
                     if (t.s[j] > 0x6000u && t.s[j] < 0x7C00u && k * PR_TS + trow < span &&
                         !((bad >> (trow >> 4)) & 1))
@@ -1064,8 +1104,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             const bool whole = k * PR_TS + PR_TS <= ss.L && bad == 0;
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int i = tid + 64 * W * j, trow = i / CR, ch = i % CR;
-                if (Stage::NP % (64 * W) && i >= Stage::NP) break;
+                const int i = tid + 64 * PR_W * j, trow = i / CR, ch = i % CR;
+                if (Stage::NP % (64 * PR_W) && i >= Stage::NP) break;
                 if constexpr (BW == 16) {
                     if (!whole) {
                         const int slot = k * PR_TS + trow;
@@ -1116,7 +1156,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             float tscale = scale;
             if constexpr (BW != 16) {
                 if (odd) { /* uniform and rare */
-                    for (int i = tid; i < Stage::NP; i += 64 * W) {
+                    for (int i = tid; i < Stage::NP; i += 64 * PR_W) {
                         const int trow = i / CR, ch = i % CR, slot = min(tb + trow, span - 1);
                         int id = tab[slot >> a.l.shift];
                         if ((unsigned)id >= (unsigned)a.l.pages) id = 0; /* masked */
@@ -1165,9 +1205,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                 return (s2p_u32x4){b0.x, b0.y, b1.x, b1.y};
             };
             if (work) {
-                read_k(0);
+                read_k(part);
 #pragma unroll
-                for (int h = 0; h < 2; h++) { /* halves of 32 slots */
+                for (int hh = 0; hh < 2 / SP; hh++) { /* halves of 32 slots */
+                    const int h = SP == 2 ? part : hh;
                     pr_f32x16 sc;
 #pragma unroll
                     for (int i = 0; i < 16; i++) sc[i] = 0.f;
@@ -1186,7 +1227,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
                         for (int dt = 0; dt < 4; dt++) vr[0][dt] = read_v(2 * h, dt);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    if (h == 0) read_k(1);
+                    if (SP == 1 && h == 0) read_k(1);
                     /* x[i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
                     float x[16];
 #pragma unroll
@@ -1305,11 +1346,46 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
             __syncthreads();
         }
         /* out, or the partial of a tile that other blocks work on too */
-        const float lt0 = pr_swap_sum(l);
+        float lt0 = pr_swap_sum(l);
+        if constexpr (SP == 2) { /* the second wave's state to the first, through the tiles' LDS */
+            LDS(s2p_f32x4)* const x01 = (LDS(s2p_f32x4)*)s_k + 512 * vw + lane;
+            LDS(s2p_f32x4)* const x23 = (LDS(s2p_f32x4)*)s_v + 512 * vw + lane;
+            if (part == 1 && busy) {
+                if (half == 0) {
+                    s_ml[vec][0] = m;
+                    s_ml[vec][1] = lt0;
+                }
+#pragma unroll
+                for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        (dt < 2 ? x01 : x23)[64 * (4 * (dt & 1) + q)] =
+                            (s2p_f32x4){o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+            }
+            __syncthreads();
+            if (part == 0 && busy) {
+                const float m1 = s_ml[vec][0], l1 = s_ml[vec][1];
+                const float mn = fmaxf(m, m1), ms = mn == -INFINITY ? 0.f : mn;
+                const float e0 = __builtin_amdgcn_exp2f(m - ms), e1 = __builtin_amdgcn_exp2f(m1 - ms);
+                lt0 = fmaf(lt0, e0, l1 * e1);
+                m = mn;
+#pragma unroll
+                for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const s2p_f32x4 z = (dt < 2 ? x01 : x23)[64 * (4 * (dt & 1) + q)];
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            o[dt][4 * q + e] = fmaf(o[dt][4 * q + e], e0, z[e] * e1);
+                    }
+            }
+            __syncthreads(); /* the next row tile's loads go there */
+        }
+        const bool leave = live && part == 0;
         const float lt = m == -INFINITY ? (any ? 1.f : 0.f) : lt0; /* -inf everywhere, not nothing */
         if (k0 == 0 && stop == last) {
             const float inv = m == -INFINITY ? (any ? NAN : 0.f) : 1.f / lt;
-            if (live) {
+            if (leave) {
                 uint16_t* out = a.out + ((size_t)row * a.qh + vhead) * PG_HD + 4 * half;
 #pragma unroll
                 for (int dt = 0; dt < 4; dt++)
@@ -1322,7 +1398,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
         } else {
             float* const po = a.work + ((size_t)(kvh * a.nb + blk) * 2 + (k0 == 0 ? 1 : 0)) *
                                            ((size_t)VEC * (PG_HD + 2));
-            if (live) {
+            if (leave) {
                 if (half == 0) {
                     po[2 * vec] = m;
                     po[2 * vec + 1] = lt;
@@ -1346,31 +1422,35 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_rows(PgAttn a) {
 }
 
 /* Row tiles that several blocks worked on, from their partials: a block a (block where the tile
- * begins, kv head, 8 vectors), four dims a thread. */
+ * begins, kv head, 8 / PARTS vectors), as in k_paged_merge. */
+template <int PARTS>
 __global__ __launch_bounds__(256) void k_paged_rows_merge(PgAttn a, int tile) {
+    constexpr int VECS = 8 / PARTS;
+    __shared__ float s_m[VECS][PARTS][3];
+    __shared__ s2p_f32x4 s_z[VECS][PARTS][32];
     const int j0 = blockIdx.z, kvh = blockIdx.y;
-    const int vec = blockIdx.x * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+    const int tid = threadIdx.x, x = tid & 31, part = (tid >> 5) % PARTS, u = (tid >> 5) / PARTS;
+    const int vec = blockIdx.x * VECS + u;
     const int row0 = a.sums[4 * j0], nvec = a.sums[4 * j0 + 1], j1 = a.sums[4 * j0 + 2];
-    if (vec >= nvec) return;
+    if ((int)blockIdx.x * VECS >= nvec) return;
+    const bool live = vec < nvec;
     const size_t stride = (size_t)tile * (PG_HD + 2);
-    const float* p = a.work + ((size_t)(kvh * a.nb + j0) * 2 + 1) * stride;
-    float M = p[2 * vec], lt = p[2 * vec + 1], mark = lt;
-    s2p_f32x4 z = *(const s2p_f32x4*)(p + 2 * tile + vec * PG_HD + d);
-    for (int j = j0 + 1; j <= j1; j++) {
-        p = a.work + (size_t)(kvh * a.nb + j) * 2 * stride;
-        const float pm = p[2 * vec], pl = p[2 * vec + 1];
-        const s2p_f32x4 pz = *(const s2p_f32x4*)(p + 2 * tile + vec * PG_HD + d);
-        const float mn = fmaxf(M, pm), ms = mn == -INFINITY ? 0.f : mn;
-        const float e0 = __builtin_amdgcn_exp2f(M - ms), e1 = __builtin_amdgcn_exp2f(pm - ms);
-        mark = fmaxf(mark, pl);
-        lt = fmaf(lt, e0, pl * e1);
-#pragma unroll
-        for (int e = 0; e < 4; e++) z[e] = fmaf(z[e], e0, pz[e] * e1);
-        M = mn;
+    PgSum o;
+    if (live)
+        o = pd_gather<PARTS>(a.work + (size_t)kvh * a.nb * 2 * stride, stride, tile, j0, j1, vec,
+                                part, 4 * x);
+    if (x == 0) {
+        s_m[u][part][0] = o.M;
+        s_m[u][part][1] = o.lt;
+        s_m[u][part][2] = o.mark;
     }
-    const float inv = M == -INFINITY ? (mark > 0.f ? NAN : 0.f) : 1.f / lt;
-    *(s2p_u32x2*)(a.out + ((size_t)(row0 + vec / a.g) * a.qh + kvh * a.g + vec % a.g) * PG_HD + d) =
-        (s2p_u32x2){pd_pk(z[0] * inv, z[1] * inv), pd_pk(z[2] * inv, z[3] * inv)};
+    s_z[u][part][x] = o.z;
+    __syncthreads();
+    if (part || !live) return;
+#pragma unroll
+    for (int i = 1; i < PARTS; i++)
+        pd_add(o, s_m[u][i][0], s_m[u][i][1], s_z[u][i][x], s_m[u][i][2]);
+    pd_out(a, row0, kvh, vec, 4 * x, o.z, o.M, o.lt, o.mark);
 }
 
 /* blocks a kv head and tile of query vectors: as many as fit at once, `each` a CU, and no more
@@ -1391,32 +1471,40 @@ static hipError_t pd_launch(PgAttn a, hipStream_t st) {
                        dim3(64 * PD_WAVES), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nb == 1 || a.b.max_len <= rnd) return e; /* no session is shared */
-    hipLaunchKernelGGL(k_paged_merge, dim3((unsigned)(a.b.max_rows * a.g), (unsigned)a.kvh,
-                                           (unsigned)a.b.sessions),
-                       dim3(512), 0, st, a, 16 * MQT);
+    hipLaunchKernelGGL(k_paged_merge, dim3((unsigned)((a.b.max_rows * a.g + PM_VECS - 1) / PM_VECS),
+                                           (unsigned)a.kvh, (unsigned)a.b.sessions),
+                       dim3(256), 0, st, a, 16 * MQT);
     return hipGetLastError();
 }
 
-template <int BW, int W>
+template <int BW, int SP>
 static hipError_t pr_launch(PgAttn a, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_rows<BW, W>), dim3((unsigned)(a.nb * a.kvh)), dim3(64 * W), 0, st, a);
+    hipLaunchKernelGGL((k_paged_rows<BW, SP>), dim3((unsigned)(a.nb * a.kvh)), dim3(64 * PR_W), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nb == 1) return e;
-    hipLaunchKernelGGL(k_paged_rows_merge, dim3(4 * W, (unsigned)a.kvh, (unsigned)a.nb), dim3(256), 0,
-                       st, a, 32 * W);
+    /* a row tile's partials: many where there are few row tiles (one session of 8,192 tokens and 17
+     * rows takes 24 us with four threads on a vector's, 31 with one; 2 x 2,048 rows, of mostly two
+     * partials, 266 and 256) */
+    constexpr int tile = 32 * PR_W / SP;
+    const int64_t tiles = (int64_t)a.b.sessions * ((a.b.max_rows + a.rt - 1) / a.rt);
+    if (a.nb > 4 * tiles)
+        hipLaunchKernelGGL((k_paged_rows_merge<4>), dim3(tile / 2, (unsigned)a.kvh, (unsigned)a.nb),
+                           dim3(256), 0, st, a, tile);
+    else
+        hipLaunchKernelGGL((k_paged_rows_merge<1>), dim3(tile / 8, (unsigned)a.kvh, (unsigned)a.nb),
+                           dim3(256), 0, st, a, tile);
     return hipGetLastError();
 }
-/* Waves of a block.  Eight read K and V half as often as four and have registers for the next
- * tile: 2 x 2,048 bf16 rows take 240 us, 300 in fours; four 17-row trees at 8,192 tokens 48 and 52.
- * Over codes four (two blocks a CU) for up to 128 query vectors, where the conversion would wait
- * for three waves' work: the trees take 58 us over INT4 codes, 72 in eights. */
-static int pr_waves(int64_t vecs, bool codes) { return codes && vecs <= 128 ? 4 : 8; }
-/* blocks a kv head over row tiles: eight waves a CU, no more than there are rounds */
-static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int g, int w) {
-    const int rt = 32 * w / g;
+/* Waves that share 32 of a row tile's vectors, each with half of a tile's slots: two where no
+ * session has more than 128 vectors, whose tiles would leave waves idle (32 sessions x 16 rows x 4
+ * heads a kv head at 300 tokens 18.3 us, 21.5 with one; four 17-row trees at 8,192 tokens over INT4
+ * codes 57 and 72) */
+static int pr_split(int64_t vecs) { return vecs <= 32 * PR_W / 2 ? 2 : 1; }
+/* blocks a kv head over row tiles of rt rows: one a CU, no more than there are rounds */
+static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int rt) {
     const int64_t most = (int64_t)b->sessions * ((b->max_rows + rt - 1) / rt) *
                          (PR_BEGIN + (b->max_len + PR_TS - 1) / PR_TS);
-    int64_t nb = 8 / w * s2p_cu_count() / kv_heads;
+    int64_t nb = s2p_cu_count() / kv_heads;
     if (nb < 1) nb = 1;
     return nb < most ? nb : most;
 }
@@ -1428,14 +1516,9 @@ extern "C" int64_t s2pk_paged_attention_work_floats(const s2p_page_batch* batch,
         return 0;
     const int64_t vecs = (int64_t)batch->max_rows * pg_group(q_heads, kv_heads);
     if (vecs > 32) {
-        const int g = pg_group(q_heads, kv_heads);
-        int64_t most = 0; /* either kind of cache */
-        for (int w = 4; w <= 8; w += 4) {
-            const int64_t nb = pr_blocks(batch, kv_heads, g, w);
-            const int64_t n = 4 * nb + kv_heads * nb * 2 * 32 * w * (PG_HD + 2);
-            if (n > most) most = n;
-        }
-        return most;
+        const int tile = 32 * PR_W / pr_split(vecs);
+        const int64_t nb = pr_blocks(batch, kv_heads, tile / pg_group(q_heads, kv_heads));
+        return 4 * nb + kv_heads * nb * 2 * tile * (PG_HD + 2);
     }
     const int64_t sums = (batch->sessions + 3) & ~3;
     return sums + kv_heads * pd_blocks(batch, kv_heads, 128, 3) * 2 * (vecs > 16 ? 32 : 16) * (PG_HD + 2);
@@ -1462,18 +1545,19 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
     a.kvh = pool->kv_heads;
     a.g = pg_group(q_heads, pool->kv_heads);
     const int64_t vecs = (int64_t)batch->max_rows * a.g;
-    const int w = pr_waves(vecs, pool->bits != 16);
-    a.rt = 32 * w / a.g;
+    const bool split = pr_split(vecs) == 2;
+    a.rt = 32 * PR_W / pr_split(vecs) / a.g;
     /* rounds are counted in 32 bits */
     if ((int64_t)batch->sessions * ((batch->max_rows + a.rt - 1) / a.rt) *
             (PR_BEGIN + (batch->max_len + PR_TS - 1) / PR_TS) > 1 << 30)
         return hipErrorInvalidValue;
     if (vecs > 32) {
-        a.nb = (int)pr_blocks(batch, a.kvh, a.g, w);
+        a.nb = (int)pr_blocks(batch, a.kvh, a.rt);
         a.work = work + 4 * (int64_t)a.nb;
-        if (w == 4) return pool->bits == 8 ? pr_launch<8, 4>(a, st) : pr_launch<4, 4>(a, st);
-        return pool->bits == 16 ? pr_launch<16, 8>(a, st)
-               : pool->bits == 8 ? pr_launch<8, 8>(a, st) : pr_launch<4, 8>(a, st);
+        if (split) return pool->bits == 16 ? pr_launch<16, 2>(a, st)
+                          : pool->bits == 8 ? pr_launch<8, 2>(a, st) : pr_launch<4, 2>(a, st);
+        return pool->bits == 16 ? pr_launch<16, 1>(a, st)
+               : pool->bits == 8 ? pr_launch<8, 1>(a, st) : pr_launch<4, 1>(a, st);
     }
     a.work = work + ((batch->sessions + 3) & ~3);
     /* 17 to 32 vectors: two tiles of them in a wave where its registers hold them.  INT4's do not
