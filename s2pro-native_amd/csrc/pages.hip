@@ -7,7 +7,13 @@
  * lowest free ids) depends on the counts alone, not on what happened before.  The
  * price is a scan of the counts, 4 bytes a page, by one workgroup.
  * Payload is moved by one launch over (page, layer, 16 KB piece) items, as many as the
- * device's list says; that copy is what bounds a fork's first tokens and a compaction. */
+ * device's list says; that copy is what bounds a fork's first tokens and a compaction.
+ * The others are bound by their chain of loads: launch, count, table, count again.
+ *
+ * MI355X, pages of 16 slots: 4 forks of 1,000 tokens 3.4 us, the reservation after them 5.9
+ * and its copies 2.9; 32 forks of 4,090 tokens at 36 layers 4.8, 7.1 and 14.6 (151 MB, read
+ * from cache); 100 of 333 pages kept and moved together: freeing 2.8 us, plan 4.1, moves 3.9;
+ * 200 pages of 36 layers (944 MB): 4.6, 5.2 and 195 (4.8 TB/s; a 2 GiB copy runs at 4.9). */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -172,8 +178,27 @@ struct PgCopy {
     int layers, kv_pieces, pieces;
 };
 
-/* one 16 KB piece of a page of a layer (or of its scales) an item */
-__global__ __launch_bounds__(256) void k_pages_copy(PgCopy c) {
+/* A compaction's new ids into the tables: to[id - live] of a page from `live` on. */
+struct PgRename {
+    s2p_page_tables t;
+    const int32_t *live, *to;
+    int pages;
+};
+S2P_DEV void pages_rename(const PgRename& r, int s) {
+    const int held = min(r.t.held[s], r.t.max_pages), live = *r.live;
+    int32_t* row = r.t.table + (size_t)s * r.t.max_pages;
+    for (int j = threadIdx.x; j < held; j += 256) {
+        const int id = row[j];
+        if (id >= live && id < r.pages) row[j] = r.to[id - live];
+    }
+}
+
+/* One 16 KB piece of a page of a layer (or of its scales) an item; RENAME: the tables too, a
+ * session a block, beside the copy (a launch of its own cost 4 us of 20). */
+template <bool RENAME>
+__global__ __launch_bounds__(256) void k_pages_copy(PgCopy c, PgRename r) {
+    if (RENAME)
+        for (int s = blockIdx.x; s < r.t.sessions; s += gridDim.x) pages_rename(r, s);
     const int64_t items = (int64_t)*c.n * c.layers * c.pieces;
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
         const int pc = (int)(it % c.pieces);
@@ -201,8 +226,9 @@ __global__ __launch_bounds__(256) void k_pages_copy(PgCopy c) {
     }
 }
 
+/* most: the pairs that there can be */
 static hipError_t copy_launch(const s2p_page_pool* p, const int32_t* n, const int32_t* src,
-                              const int32_t* dst, hipStream_t st) {
+                              const int32_t* dst, int most, const PgRename* r, hipStream_t st) {
     const size_t slots = (size_t)2 * p->kv_heads * p->page;
     PgCopy c = {};
     c.kv = (char*)p->kv;
@@ -220,7 +246,11 @@ static hipError_t copy_launch(const s2p_page_pool* p, const int32_t* n, const in
     c.src = src;
     c.dst = dst;
     c.layers = p->layers;
-    hipLaunchKernelGGL(k_pages_copy, dim3((unsigned)(8 * s2p_cu_count())), dim3(256), 0, st, c);
+    const int64_t items = (int64_t)most * p->layers * c.pieces;
+    const int64_t full = 8 * (int64_t)s2p_cu_count();
+    const dim3 grid((unsigned)(items < full ? items : full));
+    if (r) hipLaunchKernelGGL((k_pages_copy<true>), grid, dim3(256), 0, st, c, *r);
+    else hipLaunchKernelGGL((k_pages_copy<false>), grid, dim3(256), 0, st, c, PgRename{});
     return hipGetLastError();
 }
 
@@ -328,17 +358,6 @@ __global__ __launch_bounds__(PT) void k_pages_plan(int32_t* __restrict__ ref, in
     }
 }
 
-__global__ __launch_bounds__(256) void k_pages_rename(s2p_page_tables t, int pages,
-                                                      const int32_t* __restrict__ work) {
-    const int s = blockIdx.x, held = min(t.held[s], t.max_pages), live = work[1];
-    const int32_t* to = work + 4 + 2 * (pages / 2 + 1);
-    int32_t* row = t.table + (size_t)s * t.max_pages;
-    for (int j = threadIdx.x; j < held; j += 256) {
-        const int id = row[j];
-        if (id >= live && id < pages) row[j] = to[id - live];
-    }
-}
-
 static bool tables_ok(const s2p_page_pool* p, const s2p_page_tables* t) {
     return pg_pool_ok(p) && t && t->ref && t->table && t->held && t->len && t->sessions > 0 &&
            t->sessions <= S2P_PAGE_MAX_SESSIONS && t->max_pages > 0;
@@ -357,7 +376,7 @@ extern "C" hipError_t s2pk_pages_reserve(const s2p_page_pool* pool, const s2p_pa
                        pg_shift(pool->page), want, granted, work);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    return copy_launch(pool, work, work + 4, work + 4 + tab->sessions, st);
+    return copy_launch(pool, work, work + 4, work + 4 + tab->sessions, tab->sessions, nullptr, st);
 }
 
 extern "C" hipError_t s2pk_pages_fork(const s2p_page_pool* pool, const s2p_page_tables* tab,
@@ -382,11 +401,9 @@ extern "C" hipError_t s2pk_pages_compact(const s2p_page_pool* pool, const s2p_pa
                                          int32_t* n_live, int32_t* work, hipStream_t st) {
     if (!tables_ok(pool, tab) || !work) return hipErrorInvalidValue;
     hipLaunchKernelGGL(k_pages_plan, dim3(1), dim3(PT), 0, st, tab->ref, pool->pages, n_live, work);
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_pages_rename, dim3((unsigned)tab->sessions), dim3(256), 0, st, *tab,
-                       pool->pages, work);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    return copy_launch(pool, work, work + 4, work + 4 + pool->pages / 2 + 1, st);
+    const int each = pool->pages / 2 + 1; /* as k_pages_plan lays the workspace out */
+    const PgRename r = {*tab, work + 1, work + 4 + 2 * each, pool->pages};
+    return copy_launch(pool, work, work + 4, work + 4 + each, each, &r, st);
 }
