@@ -78,7 +78,7 @@ hipError_t s2pk_rope_table(s2p_bf16* tab, int n_pos, int head_dim, float rope_ba
  * rope: an s2pk_rope_table of n_pos positions.  pos: [rows] RoPE positions (a draft
  * tree's depths), or NULL: each row's slot.  A row whose position is outside the
  * table is left out.  The pages that hold the rows' slots must be the session's own
- * (s2pk_pages_reserve sees to it). */
+ * (s2pk_pages_reserve sees to it).  q lies apart from qkv. */
 hipError_t s2pk_paged_append(const s2p_page_pool* pool, const s2p_page_batch* batch, int layer,
                              const s2p_bf16* qkv, int q_heads, const s2p_bf16* qn_w,
                              const s2p_bf16* kn_w, float eps, const s2p_bf16* rope, int n_pos,
@@ -91,7 +91,7 @@ hipError_t s2pk_paged_append(const s2p_page_pool* pool, const s2p_page_batch* ba
  * are in their slots already.  A row that sees no slot gets zeros.  NaN and infinities
  * in slots that a row does not see do not reach it, and a session's bits do not depend on
  * what lies behind its last slot.  work: s2pk_paged_attention_work_floats floats, 16-byte
- * aligned.  Refused too: sessions x row tiles (max_rows in eights at worst) x 64-slot tiles
+ * aligned.  out lies apart from q.  Refused too: sessions x row tiles (max_rows in eights at worst) x 64-slot tiles
  * of max_len past 2^30. */
 hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_page_batch* batch, int layer,
                                 const s2p_bf16* q, int q_heads, const uint64_t* vis,

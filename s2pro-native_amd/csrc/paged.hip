@@ -173,7 +173,7 @@ extern "C" hipError_t s2pk_paged_append(const s2p_page_pool* pool, const s2p_pag
     if (batch && batch->rows <= 0) return hipSuccess;
     if (!pg_pool_ok(pool) || !pg_batch_ok(pool, batch) || layer < 0 || layer >= pool->layers ||
         !pg_group(q_heads, pool->kv_heads) || !qkv || !rope || !q || n_pos <= 0 ||
-        (!qn_w) != (!kn_w) ||
+        (!qn_w) != (!kn_w) || (const void*)qkv == (void*)q ||
         (((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)rope | (uintptr_t)qn_w | (uintptr_t)kn_w) & 15))
         return hipErrorInvalidValue;
     PgAppend a = {};

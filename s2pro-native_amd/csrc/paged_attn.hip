@@ -1530,7 +1530,7 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
                                            hipStream_t st) {
     if (batch && batch->rows <= 0) return hipSuccess;
     if (!pg_pool_ok(pool) || !pg_batch_ok(pool, batch) || layer < 0 || layer >= pool->layers ||
-        !pg_group(q_heads, pool->kv_heads) || !q || !out || !work ||
+        !pg_group(q_heads, pool->kv_heads) || !q || !out || !work || (const void*)q == (void*)out ||
         (((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 15) || ((uintptr_t)vis & 7) ||
         (vis && batch->max_rows > 64))
         return hipErrorInvalidValue;

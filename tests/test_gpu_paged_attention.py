@@ -315,3 +315,44 @@ def test_bits_do_not_depend_on_what_lies_behind_the_end(lib, bits, rows):
         outs.append(attend(lib, pool, b, q, kvh * g))
     for o in outs[1:]:
         assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [1, 5, 8, 20, 100])
+def test_bounds_far_above_the_lengths(lib, bits, rows):
+    """host bounds for 100,000 slots and 200 rows more than there are; 5 and 8 rows over INT8 then
+    go through two vector tiles a wave"""
+    page, kvh, g = 256, 2, 4
+    lens, n = [0, 700, 31, 255, 1000, 256, 3, 90], [rows, 1, rows, rows, 2, rows, rows, 1]
+    n = [min(x, rows) for x in n]
+    pool = Pool(61, bits, pages_for(page, lens, n), kvh, page)
+    b = new_batch(62, pool.pages, page, lens, n)
+    b.table = np.pad(b.table, ((0, 0), (0, 400 - b.table.shape[1])), constant_values=-1)
+    b.d_table = dev_i32(b.table)
+    q = rand_q(63, b.rows, kvh * g)
+    for most in (rows, rows + 200):
+        b.max_len, b.max_rows = 100_000, most
+        check(attend(lib, pool, b, q, kvh * g), *reference(pool, b, q, kvh * g), f"{most}")
+
+
+@pytest.mark.parametrize("rows", [5, 8])
+def test_two_vector_tiles_with_trees_and_unseen_values(lib, rows):
+    """INT8, 17 to 32 query vectors, enough rounds for two vector tiles a wave"""
+    page, kvh, g = 64, 4, 4
+    lens, n = [4000, 4100, 3999, 64, 0, 2500], [rows] * 6
+    pool = Pool(64, 8, pages_for(page, lens, n), kvh, page)
+    b = new_batch(65, pool.pages, page, lens, n, max_len=50_000)
+    b.table = np.pad(b.table, ((0, 0), (0, 800 - b.table.shape[1])), constant_values=-1)
+    b.table[1, 3] = pool.pages  # a page that is not there
+    b.d_table = dev_i32(b.table)
+    words = tree_words(TREE16[:rows]) * 6
+    words[2 * rows + 1] = 0  # sees the prefix alone
+    words[4 * rows + 2] = 0  # sees nothing
+    unseen = lens[3] + rows - 1
+    for i in range(rows):
+        words[3 * rows + i] &= ~(1 << (rows - 1))
+    pool.scales[0, int(b.table[3, unseen // page]), :, unseen % page] = float("nan")
+    q = rand_q(66, b.rows, kvh * g)
+    vis = keep(torch.tensor(np.array(words, np.uint64).view(np.int64), device=DEV))
+    want = reference(pool, b, q, kvh * g, words)
+    check(attend(lib, pool, b, q, kvh * g, vis), *want)

@@ -315,3 +315,69 @@ def test_a_serving_loop(lib, bits):
     assert max(p for t in m.tab for p in t) == sum(x > 0 for x in m.ref) - 1
     step([5, 0, 20, 1, 1, 3])
     step([1, 0, 1, 1, 1, 1])
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_a_captured_tick(lib, bits, rows):
+    """room, append, attention and commit of every layer in one graph: its replays are the eager
+    ticks bit for bit while the sessions grow past pages and share a prompt"""
+    kvh, g, page, layers, pages, n, width, ticks = 2, 4, 16, 2, 64, 3, 20, 12
+    qh, total = kvh * g, n * rows
+    rope = keep(torch.empty(512, 64, 2, dtype=torch.bfloat16, device=DEV))
+    s2pamd.hip_check(lib.s2pk_rope_table(P(rope), 512, HD, 1e6, S()))
+    want, row0 = dev_i32([rows] * n), dev_i32(np.arange(n + 1) * rows)
+    acc = [[(3 * t + s) % rows for s in range(n)] for t in range(ticks)]
+    path = dev_i32(np.tile(np.arange(1, rows + 1), n))
+    sides = []
+    for _ in range(2):
+        pool = Pool(5, bits, pages, kvh, page, layers)
+        d = Dev(lib, pool, n, width)
+        assert d.reserve([21, 0, 0]) == [1, 0, 0]
+        d.len.copy_(dev_i32([21, 0, 0]))
+        assert d.fork([0, 0], [1, 2]) == [1, 1]
+        b = s2pamd.PageBatch(table=d.table.data_ptr(), len=d.len.data_ptr(),
+                             row0=row0.data_ptr(), sessions=n, max_pages=width, rows=total,
+                             max_rows=rows, max_len=width * page)
+        floats = lib.s2pk_paged_attention_work_floats(ctypes.byref(b), qh, kvh)
+        sides.append(dict(
+            pool=pool, d=d, b=b, granted=dev_i32([0] * n), acc=dev_i32([0] * n),
+            qkv=keep(torch.empty(layers, total, (qh + 2 * kvh) * HD, dtype=torch.bfloat16,
+                                 device=DEV)),
+            q=keep(torch.empty(total, qh * HD, dtype=torch.bfloat16, device=DEV)),
+            out=keep(torch.empty(layers, total, qh * HD, dtype=torch.bfloat16, device=DEV)),
+            work=keep(torch.empty(floats, dtype=torch.float32, device=DEV))))
+
+    def tick(x, st):
+        d, b = x["d"], ctypes.byref(x["b"])
+        p = ctypes.byref(d.p)
+        ok = s2pamd.hip_check
+        ok(lib.s2pk_pages_reserve(p, ctypes.byref(d.t), P(want), P(x["granted"]), P(d.work), st))
+        for i in range(layers):
+            ok(lib.s2pk_paged_append(p, b, i, P(x["qkv"][i]), qh, None, None, 1e-6, P(rope), 512,
+                                     None, P(x["q"]), st))
+            ok(lib.s2pk_paged_attention(p, b, i, P(x["q"]), qh, None, P(x["out"][i]), P(x["work"]),
+                                        st))
+        ok(lib.s2pk_paged_commit(p, b, P(path), P(x["acc"]), P(d.len), st))
+
+    eager, graphed = sides
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        tick(graphed, s2pamd.stream_ptr(side))
+    for t in range(ticks):
+        new = rand_q(100 + t, layers * total, qh + 2 * kvh, 1.5)
+        for x in sides:
+            x["qkv"].copy_(new.view_as(x["qkv"]))
+            x["acc"].copy_(torch.tensor(acc[t], dtype=torch.int32))
+        torch.cuda.synchronize()
+        tick(eager, S())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert eager["granted"].tolist() == [1] * n
+        for a, b in zip((eager["d"].ref, eager["d"].table, eager["d"].len, eager["out"],
+                         eager["pool"].kv),
+                        (graphed["d"].ref, graphed["d"].table, graphed["d"].len, graphed["out"],
+                         graphed["pool"].kv)):
+            assert torch.equal(a, b), t
+    assert eager["d"].len.tolist() == [21 + sum(a[s] + 1 for a in acc) for s in range(n)]

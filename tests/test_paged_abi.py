@@ -1,13 +1,18 @@
 """The refusals of the paged-cache calls (no GPU): bad arguments are errors before
 anything is launched, no rows is success, sizes are pure functions."""
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 
 import s2pamd
 from s2pamd import PageBatch, PagePool, PageTables
 
+ROOT = Path(__file__).resolve().parent.parent
 A = 1 << 20  # an aligned address, never read
+MIRRORS = [("s2p_page_pool", PagePool), ("s2p_page_batch", PageBatch),
+           ("s2p_page_tables", PageTables)]
 
 
 @pytest.fixture(scope="module")
@@ -41,11 +46,11 @@ BAD_TABLES = [dict(ref=None), dict(table=None), dict(held=None), dict(len=None),
               dict(sessions=1025), dict(max_pages=0)]
 
 
-def attention(lib, p, b, layer=0, q=A, qh=32, vis=None, out=A, work=A):
+def attention(lib, p, b, layer=0, q=A, qh=32, vis=None, out=2 * A, work=A):
     return lib.s2pk_paged_attention(p, b, layer, q, qh, vis, out, work, None)
 
 
-def append(lib, p, b, layer=0, qkv=A, qh=32, qn=A, kn=A, rope=A, n_pos=64, q=A):
+def append(lib, p, b, layer=0, qkv=A, qh=32, qn=A, kn=A, rope=A, n_pos=64, q=2 * A):
     return lib.s2pk_paged_append(p, b, layer, qkv, qh, qn, kn, 1e-6, rope, n_pos, None, q, None)
 
 
@@ -80,7 +85,7 @@ def test_bad_tables(lib, kw):
 def test_other_arguments(lib):
     p, b, t = pool(), batch(), tables()
     for kw in (dict(layer=-1), dict(layer=2), dict(q=None), dict(q=A + 2), dict(out=None),
-               dict(out=A + 8), dict(work=None), dict(work=A + 4), dict(qh=0), dict(qh=-32),
+               dict(out=2 * A + 8), dict(work=None), dict(work=A + 4), dict(qh=0), dict(qh=-32),
                dict(qh=12), dict(qh=17 * 8), dict(vis=A + 4)):
         assert attention(lib, p, b, **kw) != 0, kw
     # visibility words have 64 bits
@@ -107,6 +112,18 @@ def test_other_arguments(lib):
         assert f(p, None, A, A, A, None) != 0
 
 
+def test_outputs_in_place_of_inputs(lib):
+    """other blocks still read the rows that one writes"""
+    assert attention(lib, pool(), batch(), q=A, out=A) != 0
+    assert append(lib, pool(), batch(), qkv=A, q=A) != 0
+
+
+def test_more_rounds_than_are_counted(lib):
+    big = dict(sessions=1024, max_pages=1 << 22, max_len=1 << 30)
+    assert attention(lib, pool(page=256), batch(**big)) != 0
+    assert lib.s2pk_paged_attention_work_floats(batch(**big), 32, 8) > 0
+
+
 def test_no_rows_is_success(lib):
     b = batch(rows=0)
     assert attention(lib, None, b) == 0
@@ -114,6 +131,25 @@ def test_no_rows_is_success(lib):
     assert lib.s2pk_paged_commit(None, b, None, None, None, None) == 0
     assert lib.s2pk_pages_fork(None, None, None, None, 0, None, None) == 0
     assert lib.s2pk_rope_table(None, 0, 128, 1e6, None) == 0
+
+
+def test_struct_mirrors(tmp_path):
+    """the ctypes mirrors lie as the header says"""
+    lines = [f'P("{c}.{f}", offsetof({c}, {f}));' for c, m in MIRRORS for f, _ in m._fields_]
+    lines += [f'P("{c}", sizeof({c}));' for c, _ in MIRRORS]
+    src = tmp_path / "layout.cpp"
+    src.write_text("#define __HIP_PLATFORM_AMD__ 1\n#include <cstdio>\n#include <s2pro/paged.h>\n"
+                   '#define P(n, v) std::printf("%s %zu\\n", n, (size_t)(v))\n'
+                   "int main() { " + "\n".join(lines) + " }\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["g++", "-std=c++17", "-w", f"-I{ROOT}/include", "-I/opt/rocm/include", str(src),
+                    "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    got = {a: int(b) for a, b in (x.split() for x in out.splitlines())}
+    for c, m in MIRRORS:
+        assert got[c] == ctypes.sizeof(m)
+        for f, _ in m._fields_:
+            assert got[f"{c}.{f}"] == getattr(m, f).offset, f
 
 
 def test_sizes(lib):
