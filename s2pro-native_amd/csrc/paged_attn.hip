@@ -1562,8 +1562,8 @@ extern "C" hipError_t s2pk_paged_attention(const s2p_page_pool* pool, const s2p_
     a.work = work + ((batch->sessions + 3) & ~3);
     /* 17 to 32 vectors: two tiles of them in a wave where its registers hold them.  INT4's do not
      * (64-slot tiles; 16 sessions x 5 rows at 8,192 tokens take 145 us so, 72 with a block for each
-     * tile); INT8's spill a little, which pays from about six rounds a block on (the same 80 and
-     * 100 us; at 1,024 tokens 33 and 30). */
+     * tile); INT8's spill a little, which pays from about six rounds a block on (8 sessions x 5 rows
+     * at 8,000 tokens 44 and 54 us; at 250 tokens 14 and 13, of 256 to 4,096 tokens 29 and 26). */
     const bool two = vecs > 16 && (pool->bits == 16 || (pool->bits == 8 &&
                      (int64_t)batch->sessions * ((batch->max_len + 127) / 128) * a.kvh >=
                          6 * 2 * (int64_t)s2p_cu_count()));

@@ -226,3 +226,28 @@ def test_commit(lib, bits):
                                            P(dev_i32([1000] * 5)), None, S()))
     for t, w in zip((pool.kv, pool.scales), want):
         assert torch.equal(t, w)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_codes_of_values_next_to_a_half(lib, table, bits):
+    """c = rint(x / s) with the f32 quotient, for values on a half step and next to it, scales that are
+    powers of two and others, down to f16's smallest"""
+    kvh, page, n, most = 4, 64, 512, 127 if bits == 8 else 7
+    rng = np.random.default_rng(bits)
+    pool = Pool(1, bits, n // page + 1, kvh, page)
+    b = new_batch(2, pool.pages, page, [0], [n])
+    top = np.exp2(rng.uniform(-26, 12, (n, kvh, 4, 1))).astype(np.float32)
+    top[::3] = most * np.exp2(rng.integers(-20, 8, (len(top[::3]), kvh, 4, 1)))
+    half = (rng.integers(-most, most, (n, kvh, 4, 32)) + 0.5) / most
+    x = np.where(rng.random(half.shape) < 0.7, half, rng.uniform(-1, 1, half.shape)) * top
+    x[..., :1] = top
+    v = torch.tensor(x.reshape(n, kvh, HD), dtype=torch.float32).to(torch.bfloat16)
+    x = v.float().numpy().reshape(n, kvh, 4, 32)
+    qkv = keep(torch.zeros(n, 3 * kvh, HD, dtype=torch.bfloat16, device=DEV))
+    qkv[:, 2 * kvh:] = v.to(DEV)
+    append(lib, pool, b, qkv.view(n, -1), kvh, None, None, table)
+    s = (np.abs(x).max(-1, keepdims=True) / np.float32(most)).astype(np.float16).astype(np.float32)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        c = np.where(s > 0, np.clip(np.rint(x / s), -most, most), 0)
+    got = np.stack([pool.values([i])[0][kvh:, p] for _, i, p in places(b)])
+    assert np.array_equal(got.reshape(x.shape), c * s.astype(np.float64))
