@@ -13,7 +13,7 @@
  * s2pk_qk_norm (elements 64, 32, 16, 8 apart across lanes, 4, 2, 1 within one), so the
  * bits are those of the separate launchers.
  *
- * MI355X, 32 query and 8 kv heads: 64 decode rows 3.2 us; 8,192 prompt rows into INT8
+ * MI355X, 32 query and 8 kv heads: 64 decode rows 3.2 us; 7,023 prompt rows into INT8
  * pages 38 us (161 MB read and written, 4.2 TB/s), of which the norm's root and
  * the codes' arithmetic are about 5. */
 #include <hip/hip_runtime.h>
