@@ -27,15 +27,17 @@
  *     so there is one barrier a tile;
  *   - O follows a new maximum only when p would pass 2^8 (f32 has the room; p's and the
  *     sums' relative precision do not depend on the maximum);
- *   - codes become K x scale in f16 (11 bits), and q, which a wave scales by a power of
- *     two, f16 without loss; V stays its exact code, its scale goes into p;
+ *   - codes become value x scale in f16 (11 bits), and q, which a wave scales by a power
+ *     of two, f16 without loss; p is f16 too, at 2^7 of itself (what is lost lies 2^-31
+ *     under the largest);
  *   - the tiles of slots that all row tiles need are dealt out evenly over one round of
  *     blocks, a row tile that several worked on is merged by k_paged_rows_merge.
  *
  * MI355X, 32 heads on 8 kv heads, in a stream of calls: 16 sessions x 8,192 tokens, one row
  * each, bf16 87 us (6.2 TB/s); 32 over INT4 codes at 512 .. 4,096 tokens 30 us; one at 100
  * tokens 5.8 us in a graph; 2 x 2,048 rows, half of them behind 2,048 tokens, 220 us
- * (770 TFLOP/s; 190 with the softmax taken out); 4 x 17 rows at 8,192 tokens 42 us. */
+ * (770 TFLOP/s; 190 with the softmax taken out); 4 x 17 rows at 8,192 tokens 41 us.  Over INT8 codes the prompt rows take 1.15 times as long
+ * (1.5 with the codes exact and p times a group's scale as its weight), the trees 45 us. */
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -913,15 +915,17 @@ template <int BW, int SP>
 __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
 #pragma clang fp contract(off)
     typedef PrStage<BW> Stage;
+    /* codes: p goes in f16, from 2^15 down to 2^-24 */
+    constexpr float SHIFT = BW == 16 ? 0.f : 7.f;
     constexpr int VEC = 32 * PR_W / SP; /* query vectors of a row tile */
     constexpr int EL = Stage::EL, NL = Stage::NL, CR = EL / 16; /* pieces of a row */
     constexpr int NC = BW == 16 ? 1 : BW == 8 ? 2 : 4;         /* 8-dim chunks of a piece */
     __shared__ __align__(256) uint16_t s_k[2][PR_TS * PG_HD], s_v[2][PR_TS * PG_HD];
     __shared__ float s_ml[SP == 2 ? VEC : 1][2];
     __shared__ int s_pre[S2P_PAGE_MAX_SESSIONS], s_w[PR_W];
-    /* bf16: nodes whose V holds a NaN or infinity; codes: a K scale over 512 */
+    /* of a tile: nodes whose V holds a NaN or infinity; codes: a scale over 512 */
     __shared__ unsigned long long s_odd[3];
-    __shared__ __align__(16) uint16_t s_vs[BW == 16 ? 1 : 2][PR_TS][4]; /* codes: V scales */
+    __shared__ int s_big[3];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, col = lane & 31;
@@ -952,7 +956,7 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
         if (base + tid < a.b.sessions) s_pre[base + tid] = total + v;
         total = all;
     }
-    if (tid < 3) s_odd[tid] = 0;
+    if (tid < 3) s_odd[tid] = s_big[tid] = 0;
     __syncthreads();
     const int nb = min(a.nb, total);
     if (blk >= nb) {
@@ -1069,12 +1073,12 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
         auto bad_of = [&](int k) __attribute__((always_inline)) {
             return (int)((__ballot(ids < 0) >> (((k - k0) & 15) * 4)) & 15);
         };
-        /* tile k to LDS.  Codes: K x scale in f16 (2^-12 off; a tile with a scale over 512 is marked
-         * and brought again as 2^-7 of itself, which stays in range), V's codes in bf16 (exact) and
-         * their scales.  bf16: V rows that are not there become zeros (what lies there may be NaN,
-         * and 0 x NaN is NaN), and so do pieces of a node's V with a NaN or infinity, which the rows
-         * that see the node add by themselves. */
-        auto put_k = [&](s2p_u32x4 w16, float ks, int trow, int ch, int buf) __attribute__((always_inline)) {
+        /* Tile k to LDS.  Codes: value x scale in f16 (2^-12 off; a tile with a scale over 512 is
+         * marked and brought again as 2^-7 of itself, which stays in range).  V rows that are not
+         * there become zeros (what lies there may be NaN, and 0 x NaN is NaN), and so do pieces of a
+         * node's V with a NaN or infinity, which the rows that see the node add by themselves. */
+        auto put = [&](s2p_u32x4 w16, float sc, LDS(uint16_t)* to, int trow, int ch, bool is_v)
+                       __attribute__((always_inline)) {
 #pragma unroll
             for (int e = 0; e < NC; e++) {
                 s2p_u32x4 w = w16;
@@ -1082,22 +1086,22 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const uint32_t x = BW == 8 ? w16[2 * e + (q >> 1)] : w16[e];
-                        w[q] = pr_pk_f16(pr_code<BW>(x, q, 0) * ks, pr_code<BW>(x, q, 1) * ks);
+                        w[q] = pr_pk_f16(pr_code<BW>(x, q, 0) * sc, pr_code<BW>(x, q, 1) * sc);
                     }
                 }
-                *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_k[buf] + pr_koff(trow, NC * ch + e)) = w;
+                *(LDS(s2p_u32x4)*)(to + (is_v ? pr_voff(trow, NC * ch + e) : pr_koff(trow, NC * ch + e))) = w;
             }
         };
+        auto big = [&](uint16_t sc) { return sc > 0x6000u && sc < 0x7C00u; }; /* 512 < sc < inf */
         auto store_k = [&](Stage& t, int k, int buf, int bad, int slot3) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int i = tid + 64 * PR_W * j, trow = i / CR, ch = i % CR;
                 if (Stage::NP % (64 * PR_W) && i >= Stage::NP) break;
-                if constexpr (BW != 16) /* 512 < scale < inf, in a slot that is there */
-                    if (t.s[j] > 0x6000u && t.s[j] < 0x7C00u && k * PR_TS + trow < span &&
-                        !((bad >> (trow >> 4)) & 1))
-                        s_odd[slot3] = 1;
-                put_k(t.w[j], BW == 16 ? 1.f : h2f(t.s[j]), trow, ch, buf);
+                if constexpr (BW != 16) /* in a slot that is there */
+                    if (big(t.s[j]) && k * PR_TS + trow < span && !((bad >> (trow >> 4)) & 1))
+                        s_big[slot3] = 1;
+                put(t.w[j], BW == 16 ? 1.f : h2f(t.s[j]), (LDS(uint16_t)*)s_k[buf], trow, ch, false);
             }
         };
         auto store_v = [&](Stage& t, int k, int buf, int bad, int slot3) __attribute__((always_inline)) {
@@ -1106,29 +1110,20 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
             for (int j = 0; j < NL; j++) {
                 const int i = tid + 64 * PR_W * j, trow = i / CR, ch = i % CR;
                 if (Stage::NP % (64 * PR_W) && i >= Stage::NP) break;
-                if constexpr (BW == 16) {
-                    if (!whole) {
-                        const int slot = k * PR_TS + trow;
-                        const bool gone = slot >= ss.L + ss.n || ((bad >> (trow >> 4)) & 1);
-                        const bool odd = !gone && slot >= ss.L && pr_odd(t.w[j]);
-                        if (gone || odd) t.w[j] = (s2p_u32x4){0u, 0u, 0u, 0u};
-                        if (odd) atomicOr(&s_odd[slot3], 1ull << trow);
+                if (!whole) {
+                    const int slot = k * PR_TS + trow;
+                    const bool gone = slot >= ss.L + ss.n || ((bad >> (trow >> 4)) & 1);
+                    const bool odd = !gone && slot >= ss.L &&
+                                     (BW == 16 ? pr_odd(t.w[j]) : (t.s[j] & 0x7C00u) == 0x7C00u);
+                    if (gone || odd) {
+                        t.w[j] = (s2p_u32x4){0u, 0u, 0u, 0u};
+                        if constexpr (BW != 16) t.s[j] = 0;
                     }
-                } else {
-                    if (BW == 4 || !(ch & 1)) s_vs[buf][trow][BW == 4 ? ch : ch >> 1] = t.s[j];
+                    if (odd) atomicOr(&s_odd[slot3], 1ull << trow);
                 }
-#pragma unroll
-                for (int e = 0; e < NC; e++) {
-                    s2p_u32x4 w = t.w[j];
-                    if constexpr (BW != 16) {
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint32_t x = BW == 8 ? t.w[j][2 * e + (q >> 1)] : t.w[j][e];
-                            w[q] = pd_pk(pr_code<BW>(x, q, 0), pr_code<BW>(x, q, 1));
-                        }
-                    }
-                    *(LDS(s2p_u32x4)*)((LDS(uint16_t)*)s_v[buf] + pr_voff(trow, NC * ch + e)) = w;
-                }
+                if constexpr (BW != 16)
+                    if (big(t.s[j]) && k * PR_TS + trow < span) s_big[slot3] = 1;
+                put(t.w[j], BW == 16 ? 1.f : h2f(t.s[j]), (LDS(uint16_t)*)s_v[buf], trow, ch, true);
             }
         };
 
@@ -1152,23 +1147,33 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
             const LDS(uint16_t)* vt = (const LDS(uint16_t)*)s_v[buf];
             const int after = seq == 2 ? 0 : seq + 1;
             const unsigned long long odd = s_odd[seq];
-            if (tid == 0) s_odd[seq ? seq - 1 : 2] = 0; /* everybody has read it, nobody set it again */
+            bool down = false; /* the tile's K and V are 2^-7 of themselves */
             float tscale = scale;
             if constexpr (BW != 16) {
-                if (odd) { /* uniform and rare */
+                down = s_big[seq] != 0;
+                if (down) { /* uniform and rare */
                     for (int i = tid; i < Stage::NP; i += 64 * PR_W) {
                         const int trow = i / CR, ch = i % CR, slot = min(tb + trow, span - 1);
                         int id = tab[slot >> a.l.shift];
-                        if ((unsigned)id >= (unsigned)a.l.pages) id = 0; /* masked */
+                        const bool there = tb + trow < span && (unsigned)id < (unsigned)a.l.pages;
+                        if (!there) id = 0; /* masked */
                         const size_t at = (((size_t)id * a.l.planes + kvh) << a.l.shift) +
                                           (slot & (a.l.page - 1));
-                        const float ks = h2f(a.l.sc[at * 4 + (BW == 8 ? ch >> 1 : ch)]);
-                        put_k(*(const s2p_u32x4*)(a.l.kv + at * EL + 16 * ch), ks * 0.0078125f, trow, ch, buf);
+                        const size_t av = at + ((size_t)a.kvh << a.l.shift);
+                        const int gp = BW == 8 ? ch >> 1 : ch;
+                        put(*(const s2p_u32x4*)(a.l.kv + at * EL + 16 * ch),
+                            h2f(a.l.sc[at * 4 + gp]) * 0.0078125f, (LDS(uint16_t)*)s_k[buf], trow, ch, false);
+                        uint16_t vs = a.l.sc[av * 4 + gp];
+                        if (!there || (slot >= ss.L && (vs & 0x7C00u) == 0x7C00u)) vs = 0;
+                        put(*(const s2p_u32x4*)(a.l.kv + av * EL + 16 * ch), h2f(vs) * 0.0078125f,
+                            (LDS(uint16_t)*)s_v[buf], trow, ch, true);
                     }
                     tscale = scale * 128.0f;
                     __syncthreads();
                 }
             }
+            /* the marks of the tile before: everybody has read them, nobody has set them again */
+            if (tid == 0) s_odd[seq ? seq - 1 : 2] = s_big[seq ? seq - 1 : 2] = 0;
             const bool work = busy && tb < wend;
             const bool open = tb + PR_TS <= open_end && bad == 0;
             uint64_t seen = ~0ull;
@@ -1222,11 +1227,9 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
                     __builtin_amdgcn_sched_barrier(0);
                     /* the next operands are read while the softmax runs */
                     s2p_u32x4 vr[2][4];
-                    if constexpr (BW == 16) {
 #pragma unroll
-                        for (int dt = 0; dt < 4; dt++) vr[0][dt] = read_v(2 * h, dt);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                    for (int dt = 0; dt < 4; dt++) vr[0][dt] = read_v(2 * h, dt);
+                    __builtin_amdgcn_sched_barrier(0);
                     if (SP == 1 && h == 0) read_k(1);
                     /* x[i]: slot 32 h + 8 (i / 4) + 4 half + i % 4 of this lane's vector */
                     float x[16];
@@ -1250,7 +1253,7 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
                         for (int dt = 0; dt < 4; dt++) o[dt] *= corr;
                         m = mn;
                     }
-                    const float ms = m == -INFINITY ? 0.f : m;
+                    const float ms = m == -INFINITY ? 0.f : m - SHIFT;
                     float ls = 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -1258,76 +1261,73 @@ __global__ __launch_bounds__(64 * PR_W, 2) void k_paged_rows(PgAttn a) {
                         ls += x[i];
                     }
                     l += ls;
-                    if constexpr (BW == 16) {
-                        if (odd) { /* uniform and rare: what store_v left out, from the page */
-                            for (uint32_t w = (uint32_t)(odd >> (32 * h)); w; w &= w - 1) {
-                                const int t = __ffs(w) - 1, slot = tb + 32 * h + t;
-                                float p = 0.f;
+                    if (odd) { /* uniform and rare: what store_v left out, from the page */
+                        for (uint32_t w = (uint32_t)(odd >> (32 * h)); w; w &= w - 1) {
+                            const int t = __ffs(w) - 1, slot = tb + 32 * h + t;
+                            float p = 0.f;
 #pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    p = (t >> 3) == (i >> 2) && (t & 3) == (i & 3) ? x[i] : p;
-                                p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
-                                if ((seen >> (32 * h + t)) & 1) {
-                                    const int id = tab[slot >> a.l.shift]; /* there: its bit is set */
-                                    const char* vp = a.l.kv +
-                                        ((((size_t)id * a.l.planes + a.kvh + kvh) << a.l.shift) +
-                                         (slot & (a.l.page - 1))) * EL;
+                            for (int i = 0; i < 16; i++)
+                                p = (t >> 3) == (i >> 2) && (t & 3) == (i & 3) ? x[i] : p;
+                            p = __shfl(p, ((t >> 2) & 1) * 32 + col, 64);
+                            if ((seen >> (32 * h + t)) & 1) {
+                                const int id = tab[slot >> a.l.shift]; /* there: its bit is set */
+                                const size_t at = (((size_t)id * a.l.planes + a.kvh + kvh) << a.l.shift) +
+                                                  (slot & (a.l.page - 1));
+                                const char* vp = a.l.kv + at * EL;
 #pragma unroll
-                                    for (int i = 0; i < 16; i++) { /* o[i / 4], dims 8 (i % 4) + 4 half .. */
-                                        const s2p_u32x4 w8 = *(const s2p_u32x4*)(vp + 64 * (i >> 2) + 16 * (i & 3));
+                                for (int i = 0; i < 16; i++) { /* o[i / 4], dims 8 (i % 4) + 4 half .. */
+                                    float v[4];
+                                    if constexpr (BW == 16) {
+                                        const s2p_u32x4 w8 =
+                                            *(const s2p_u32x4*)(vp + 64 * (i >> 2) + 16 * (i & 3));
                                         if (!pr_odd(w8)) continue;
 #pragma unroll
                                         for (int e = 0; e < 4; e++) {
                                             const uint32_t d = half ? w8[2 + (e >> 1)] : w8[e >> 1];
-                                            o[i >> 2][4 * (i & 3) + e] =
-                                                fmaf(p, e & 1 ? bf2f_hi(d) : bf2f_lo(d), o[i >> 2][4 * (i & 3) + e]);
+                                            v[e] = e & 1 ? bf2f_hi(d) : bf2f_lo(d);
+                                        }
+                                    } else {
+                                        const uint16_t vs = a.l.sc[at * 4 + (i >> 2)];
+                                        if ((vs & 0x7C00u) != 0x7C00u) continue;
+                                        const int d = 32 * (i >> 2) + 8 * (i & 3) + 4 * half;
+#pragma unroll
+                                        for (int e = 0; e < 4; e++) {
+                                            const int byte = (int8_t)vp[BW == 8 ? d + e : (d + e) >> 1];
+                                            const int c = BW == 8 ? byte
+                                                          : e & 1 ? byte >> 4 : (int)((uint32_t)byte << 28) >> 28;
+                                            v[e] = (float)c * h2f(vs);
                                         }
                                     }
+#pragma unroll
+                                    for (int e = 0; e < 4; e++)
+                                        o[i >> 2][4 * (i & 3) + e] =
+                                            fmaf(p, v[e], o[i >> 2][4 * (i & 3) + e]);
                                 }
                             }
                         }
+                    }
+                    if (BW != 16 && down) {
 #pragma unroll
-                        for (int dt = 0; dt < 4; dt++) vr[1][dt] = read_v(2 * h + 1, dt);
-                        __builtin_amdgcn_sched_barrier(0);
+                        for (int dt = 0; dt < 4; dt++) o[dt] *= 0.0078125f;
+                    }
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            const s2p_u32x4 pw = {pd_pk(x[8 * b], x[8 * b + 1]), pd_pk(x[8 * b + 2], x[8 * b + 3]),
-                                                  pd_pk(x[8 * b + 4], x[8 * b + 5]), pd_pk(x[8 * b + 6], x[8 * b + 7])};
+                    for (int dt = 0; dt < 4; dt++) vr[1][dt] = read_v(2 * h + 1, dt);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int dt = 0; dt < 4; dt++) o[dt] = mfma32x32x16(vr[b][dt], pw, o[dt]);
-                        }
-                    } else {
-                        /* a scale group is a tile of 32 dims: p times the group's scale is its weight */
+                    for (int b = 0; b < 2; b++) {
+                        s2p_u32x4 pw;
 #pragma unroll
-                        for (int gp = 0; gp < 2; gp++) {
-                            uint32_t vs[16]; /* scales of groups 2 gp, 2 gp + 1 of x[i]'s slot */
+                        for (int e = 0; e < 4; e++)
+                            pw[e] = BW == 16 ? pd_pk(x[8 * b + 2 * e], x[8 * b + 2 * e + 1])
+                                             : pr_pk_f16(x[8 * b + 2 * e], x[8 * b + 2 * e + 1]);
 #pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                vs[i] = *(const LDS(uint32_t)*)((const LDS(uint16_t)*)&s_vs[buf][0][0] +
-                                                                4 * (32 * h + 8 * (i >> 2) + 4 * half + (i & 3)) + 2 * gp);
+                        for (int dt = 0; dt < 4; dt++)
+                            o[dt] = BW == 16 ? mfma32x32x16(vr[b][dt], pw, o[dt])
+                                             : mfma32x32x16_f16(vr[b][dt], pw, o[dt]);
+                    }
+                    if (BW != 16 && down) {
 #pragma unroll
-                            for (int g = 0; g < 2; g++) {
-                                const int dt = 2 * gp + g;
-                                s2p_u32x4 va[2];
-#pragma unroll
-                                for (int b = 0; b < 2; b++) va[b] = read_v(2 * h + b, dt);
-                                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                                for (int b = 0; b < 2; b++) {
-                                    s2p_u32x4 pw;
-#pragma unroll
-                                    for (int e = 0; e < 4; e++) {
-                                        const int i = 8 * b + 2 * e;
-                                        pw[e] = pd_pk(fmaf(pd_half(vs[i], g), x[i], 0.f),
-                                                      fmaf(pd_half(vs[i + 1], g), x[i + 1], 0.f));
-                                        if (!open) /* a scale may be NaN where the slot is not seen */
-                                            pw[e] &= ((mine >> (8 * (i >> 2) + (i & 3))) & 1 ? 0xFFFFu : 0u) |
-                                                     ((mine >> (8 * (i >> 2) + (i & 3) + 1)) & 1 ? 0xFFFF0000u : 0u);
-                                    }
-                                    o[dt] = mfma32x32x16(va[b], pw, o[dt]);
-                                }
-                            }
-                        }
+                        for (int dt = 0; dt < 4; dt++) o[dt] *= 128.0f;
                     }
                 }
             }
@@ -1497,8 +1497,7 @@ static hipError_t pr_launch(PgAttn a, hipStream_t st) {
 }
 /* Waves that share 32 of a row tile's vectors, each with half of a tile's slots: two where no
  * session has more than 128 vectors, whose tiles would leave waves idle (32 sessions x 16 rows x 4
- * heads a kv head at 300 tokens 18.3 us, 21.5 with one; four 17-row trees at 8,192 tokens over INT4
- * codes 57 and 72) */
+ * heads a kv head at 300 tokens 18.3 us, 21.5 with one) */
 static int pr_split(int64_t vecs) { return vecs <= 32 * PR_W / 2 ? 2 : 1; }
 /* blocks a kv head over row tiles of rt rows: one a CU, no more than there are rounds */
 static int64_t pr_blocks(const s2p_page_batch* b, int kv_heads, int rt) {

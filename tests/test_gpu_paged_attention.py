@@ -8,7 +8,7 @@ import torch
 
 import s2pamd
 from gpu_util import DEV, P, to_host
-from paged_util import (Batch, Pool, attend, check, dev_i32, keep, new_batch, pages_for, rand_q,
+from paged_util import (HD, Batch, Pool, attend, check, dev_i32, keep, new_batch, pages_for, rand_q,
                         reference, tree_words)
 
 pytestmark = pytest.mark.gpu
@@ -356,3 +356,30 @@ def test_two_vector_tiles_with_trees_and_unseen_values(lib, rows):
     vis = keep(torch.tensor(np.array(words, np.uint64).view(np.int64), device=DEV))
     want = reference(pool, b, q, kvh * g, words)
     check(attend(lib, pool, b, q, kvh * g, vis), *want)
+
+
+@pytest.mark.parametrize("bits,rows", [(8, 1), (4, 5), (8, 40), (4, 40), (8, 100), (4, 100)])
+@pytest.mark.parametrize("vscale", [2.0 ** 14, 2.0 ** 9, 2.0 ** -12])
+def test_far_off_values_of_codes(lib, bits, rows, vscale):
+    """V scales of hundreds in the prefix, among the nodes and alone in a tile, and tiny ones; some
+    groups only, so that a tile holds both; a NaN and an infinite scale that one row's view leaves out"""
+    page, kvh, g = 32, 2, 4
+    lens, n = [150, 20], [rows, min(rows, 3)]
+    pool = Pool(71, bits, pages_for(page, lens, n), kvh, page)
+    b = new_batch(72, pool.pages, page, lens, n)
+    v = pool.scales[0, :, kvh:]
+    v[:, :, ::3, 1:3] = (v[:, :, ::3, 1:3].float() * vscale).to(torch.float16)
+    last = lens[0] + rows - 1
+    bad = pool.scales[0, int(b.table[0, last // page]), kvh:, last % page]
+    bad[0, 2], bad[1, 0] = float("nan"), float("inf")
+    q = rand_q(73, b.rows, kvh * g)
+    out = attend(lib, pool, b, q, kvh * g)
+    with np.errstate(invalid="ignore"):
+        want, tol = reference(pool, b, q, kvh * g)
+    seen = rows - 1  # the one row that sees the bad scales
+    got = out.float().view(b.rows, kvh, g, HD).cpu()
+    assert torch.isnan(got[seen, 0, :, 64:96]).all()
+    assert not torch.isfinite(got[seen, 1, :, :32]).any()
+    keep_rows = [i for i in range(b.rows) if i != seen]
+    flat = torch.tensor(keep_rows, device=DEV)
+    check(out[flat], want[keep_rows], tol[keep_rows], f"{vscale}")
